@@ -91,6 +91,23 @@ static inline WView wview(const hd_weight *w) {
     return WView{w->q, w->aux, w->meta, w->dsb, w->rows, w->units};
 }
 
+// Makes the context's device current for the length of a scope.
+struct HdDevice {
+    int before = -1;
+    explicit HdDevice(const hd_ctx *ctx) {
+        int d = -1;
+        if (cudaGetDevice(&d) == cudaSuccess && d != ctx->device) {
+            before = d;
+            cudaSetDevice(ctx->device);
+        }
+    }
+    ~HdDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+    HdDevice(const HdDevice &) = delete;
+    HdDevice &operator=(const HdDevice &) = delete;
+};
+
 // ------------------------------------------------------------------ errors
 int hd_fail(hd_ctx *ctx, int code, const char *fmt, ...);
 #define HD_CUDA_TRY(ctx, expr)                                                         \
@@ -164,6 +181,9 @@ int hd_qgemv_tc(hd_ctx *ctx, const hd_weight *w, const float *x, float *y, int B
 // and v appended to cache sequence r / T at position pos[r].
 int hd_rope_kv_append(hd_ctx *ctx, float *qkv, int64_t ld, const int32_t *pos, int rows, int T, int n_heads, int n_kv,
                       int hd, float *kc, float *vc, int max_ctx);
+
+// The 4-bit cache's shape, as every entry point over it wants it (hd_kv4.cu).
+int hd_kv4_check(hd_ctx *ctx, const char *name, const void *cache, int64_t pages, int page_size, int n_kv, int head_dim);
 
 // Launch with programmatic stream serialization, so the next kernel's
 // pre-dependency prologue (weight prefetch) overlaps this one's tail.

@@ -39,6 +39,8 @@ EXPORTS = [
     "hd_kv_arena_create", "hd_kv_arena_free", "hd_kv_layer", "hd_kv_allocate", "hd_kv_release", "hd_kv_session",
     "hd_kv_advance", "hd_kv_soul_sessions", "hd_kv_snapshot", "hd_kv_restore", "hd_kv_snapshot_free",
     "hd_kv_append_slots", "hd_attention_decode_slots", "hd_quantize_q8_1", "hd_qgemv_q8_1",
+    "hd_sample_filtered", "hd_kv_pages_assign", "hd_kv_pages_release", "hd_kv4_cache_bytes", "hd_kv4_append", "hd_kv4_read",
+    "hd_kv4_workspace_bytes", "hd_kv4_attention_decode", "hd_kv4_attention_prefill",
 ]
 
 
@@ -106,6 +108,14 @@ def lib() -> C.CDLL:
         "hd_kv_append_slots": [V, V, V, V, V, V, V, I, I, I, I],
         "hd_attention_decode_slots": [V, V, V, V, V, V, I, I, I, I, I, V],
         "hd_quantize_q8_1": [V, V, I, I64, V], "hd_qgemv_q8_1": [V, V, V, V, I],
+        "hd_sample_filtered": [V, V, I64, I64, I64, V, V, V, V, V, V],
+        "hd_kv_pages_assign": [V, V, V, I, V, I, I, I, V, V, V, V, V, V, V, I64, V],
+        "hd_kv_pages_release": [V, V, V, I, V, I, I, V, V, I, V],
+        "hd_kv4_cache_bytes": [I64, I, I, I], "hd_kv4_workspace_bytes": [V, I, I, I],
+        "hd_kv4_append": [V, V, V, I64, I64, V, I64, I, I, V, I64, I],
+        "hd_kv4_read": [V, V, I64, I, V, I64, I, I, V, V],
+        "hd_kv4_attention_decode": [V, V, I64, V, I64, I, V, I, V, I, I, I, I, I, I, F, V, V, SZ],
+        "hd_kv4_attention_prefill": [V, V, I64, V, I64, I, V, I, V, V, I, I64, I, I, I, I, I, F, V],
     }
     for name, args in sig.items():
         fn = getattr(L, name)
@@ -114,7 +124,8 @@ def lib() -> C.CDLL:
     L.hd_last_error.restype = C.c_char_p
     L.hd_gguf_error.restype = C.c_char_p
     L.hd_version.restype = C.c_char_p
-    L.hd_ctx_launch_count.restype = C.c_uint64
+    for name in ("hd_ctx_launch_count", "hd_kv4_cache_bytes", "hd_kv4_workspace_bytes"):
+        getattr(L, name).restype = C.c_uint64
     _lib = L
     return L
 
@@ -125,6 +136,32 @@ def _ptr(t) -> int | None:
     if isinstance(t, np.ndarray):
         return t.ctypes.data
     return t.data_ptr()
+
+
+def _f32_rows(t, name: str) -> int:
+    """Row stride of a float32 tensor whose rows are dense."""
+    import torch
+
+    if t.dtype != torch.float32 or t[0].numel() > 1 and not t[0].is_contiguous():
+        raise ValueError(f"{name} must be float32 with dense rows")
+    return t.stride(0)
+
+
+def _dense(dtype_name: str, **tensors):
+    """Every given tensor is dense and of the dtype."""
+    import torch
+
+    dtype = getattr(torch, dtype_name)
+    for name, t in tensors.items():
+        if t is not None and (t.dtype != dtype or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a dense {dtype_name} tensor")
+
+
+def kv4_cache_shape(pages: int, page_size: int, n_kv: int, head_dim: int) -> tuple[int, int, int, int]:
+    """Shape of a layer's 4-bit cache as a uint8 tensor."""
+    if not lib().hd_kv4_cache_bytes(pages, page_size, n_kv, head_dim) and pages:
+        raise ValueError(f"no 4-bit cache of page size {page_size}, {n_kv} kv heads, head_dim {head_dim}")
+    return pages, n_kv, page_size // 16, 18 * head_dim
 
 
 class Weight:
@@ -224,6 +261,111 @@ class Context:
         """One index per row of [rows, n] logits into int32 idx[rows]."""
         rows, n = (1, logits.numel()) if logits.dim() == 1 else logits.shape
         self._check(lib().hd_sample_rows(self.h, _ptr(logits), rows, n, seed, offset, _ptr(idx)))
+
+    def sample_filtered(self, logits, u, idx, temperature=None, top_k=None, top_p=None, min_p=None):
+        """One int32 index per row of float32 logits [rows, n] (rows may be
+        strided) from u [rows] in [0, 1), after temperature, top-k, top-p and
+        min-p; the settings are [rows] tensors (top_k int32) or None."""
+        _dense("float32", u=u, temperature=temperature, top_p=top_p, min_p=min_p)
+        _dense("int32", idx=idx, top_k=top_k)
+        rows, n = logits.shape
+        if any(t is not None and t.numel() != rows for t in (u, idx, temperature, top_k, top_p, min_p)):
+            raise ValueError(f"u, idx and the settings must have one entry for each of the {rows} rows")
+        ld = _f32_rows(logits, "logits") if rows else n
+        self._check(lib().hd_sample_filtered(self.h, _ptr(logits), ld if rows > 1 else n, rows, n, _ptr(temperature),
+                                             _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u), _ptr(idx)))
+
+    # ---- paged KV cache ----
+    def kv_pages_assign(self, lens, new, tables, page_size: int, pages: int, free, n_free, n_free_out, lens_out, row0, slots,
+                        pos, status):
+        """Places new[r] tokens of each request (hd_kv_pages_assign); every
+        argument an int32 device tensor, tables [reqs, max_pages], slots and
+        pos [max_rows]; n_free_out / lens_out may be n_free / lens."""
+        _dense("int32", lens=lens, new=new, tables=tables, free=free, n_free=n_free, n_free_out=n_free_out, lens_out=lens_out,
+               row0=row0, slots=slots, pos=pos, status=status)
+        reqs, width = tables.shape
+        if lens.numel() != reqs or new.numel() != reqs or lens_out.numel() != reqs or row0.numel() != reqs + 1 or \
+                slots.numel() != pos.numel():
+            raise ValueError(f"lens, new, lens_out, row0, slots or pos do not fit {reqs} requests")
+        self._check(lib().hd_kv_pages_assign(self.h, _ptr(lens), _ptr(new), reqs, _ptr(tables), width, page_size, pages,
+                                             _ptr(free), _ptr(n_free), _ptr(n_free_out), _ptr(lens_out), _ptr(row0),
+                                             _ptr(slots), _ptr(pos), slots.numel(), _ptr(status)))
+
+    def kv_pages_release(self, done, lens, tables, page_size: int, free, n_free, status):
+        """Gives back the pages of the requests with done[r] != 0."""
+        _dense("int32", done=done, lens=lens, tables=tables, free=free, n_free=n_free, status=status)
+        reqs, width = tables.shape
+        if lens.numel() != reqs or done.numel() != reqs:
+            raise ValueError(f"lens or done do not fit {reqs} requests")
+        self._check(lib().hd_kv_pages_release(self.h, _ptr(done), _ptr(lens), reqs, _ptr(tables), width, page_size, _ptr(free),
+                                              _ptr(n_free), free.numel(), _ptr(status)))
+
+    @staticmethod
+    def _kv4_shape(cache):
+        """(pages, page_size, n_kv, head_dim) of a uint8 cache tensor [pages, n_kv, page_size / 16, 18 * head_dim]."""
+        _dense("uint8", cache=cache)
+        if cache.dim() != 4 or cache.shape[3] % 18:
+            raise ValueError("cache must be [pages, n_kv, page_size / 16, 18 * head_dim]")
+        pages, n_kv, tiles, width = cache.shape
+        return pages, 16 * tiles, n_kv, width // 18
+
+    def kv4_append(self, k, v, slots, cache):
+        """k, v [rows, n_kv, head_dim] (rows may be strided) quantized into the cache's slots."""
+        pages, page, n_kv, hd = self._kv4_shape(cache)
+        rows = slots.numel()
+        _dense("int32", slots=slots)
+        if k.shape[0] != rows or v.shape[0] != rows or k.numel() != rows * n_kv * hd or v.numel() != k.numel():
+            raise ValueError("k, v, slots and cache do not fit")
+        if rows:
+            self._check(lib().hd_kv4_append(self.h, _ptr(k), _ptr(v), _f32_rows(k, "k") if rows > 1 else 0,
+                                            _f32_rows(v, "v") if rows > 1 else 0, _ptr(slots), rows, n_kv, hd, _ptr(cache),
+                                            pages, page))
+
+    def kv4_read(self, cache, slots, k, v):
+        """The values that slots hold into k, v [rows, n_kv, head_dim]."""
+        pages, page, n_kv, hd = self._kv4_shape(cache)
+        _dense("int32", slots=slots)
+        _dense("float32", k=k, v=v)
+        if k.numel() != slots.numel() * n_kv * hd or v.numel() != k.numel():
+            raise ValueError("k, v, slots and cache do not fit")
+        self._check(lib().hd_kv4_read(self.h, _ptr(cache), pages, page, _ptr(slots), slots.numel(), n_kv, hd, _ptr(k),
+                                      _ptr(v)))
+
+    def kv4_workspace_bytes(self, n_heads: int, n_kv: int, head_dim: int) -> int:
+        return int(lib().hd_kv4_workspace_bytes(self.h, n_heads, n_kv, head_dim))
+
+    def _kv4_rows(self, q, cache, tables, lens, out, n_lens):
+        shape = self._kv4_shape(cache)
+        _dense("int32", tables=tables, lens=lens)
+        _dense("float32", out=out)
+        if tables.dim() != 2 or tables.shape[0] != n_lens or lens.numel() != n_lens or out.numel() != q.numel() or \
+                q.numel() % (max(1, q.shape[0]) * shape[3]):
+            raise ValueError("q, cache, tables, lens and out do not fit")
+        heads = q.numel() // max(1, q.shape[0]) // shape[3]
+        return shape, heads, _f32_rows(q, "q") if q.shape[0] > 1 else 0
+
+    def kv4_attention_decode(self, q, cache, tables, lens, out, window: int = 0, sinks: int = 0, scale: float = 0.0, ws=None):
+        """q [seqs, heads, head_dim] (rows may be strided): each request's last
+        position against its cached ones.  ws: a zeroed uint8 tensor of
+        kv4_workspace_bytes, or None for the context's own."""
+        if not q.shape[0]:
+            return
+        (pages, page, n_kv, hd), heads, ld = self._kv4_rows(q, cache, tables, lens, out, q.shape[0])
+        self._check(lib().hd_kv4_attention_decode(self.h, _ptr(q), ld, _ptr(cache), pages, page, _ptr(tables), tables.shape[1],
+                                                  _ptr(lens), lens.numel(), heads, n_kv, hd, window, sinks, scale, _ptr(out),
+                                                  _ptr(ws), ws.numel() if ws is not None else 0))
+
+    def kv4_attention_prefill(self, q, cache, tables, lens, row0, out, window: int = 0, sinks: int = 0, scale: float = 0.0):
+        """q [rows, heads, head_dim]: rows row0[r] .. row0[r+1]-1 are request r's last positions."""
+        if not q.shape[0]:
+            return
+        (pages, page, n_kv, hd), heads, ld = self._kv4_rows(q, cache, tables, lens, out, lens.numel())
+        _dense("int32", row0=row0)
+        if row0.numel() != lens.numel() + 1:
+            raise ValueError("row0 must have one more entry than lens")
+        self._check(lib().hd_kv4_attention_prefill(self.h, _ptr(q), ld, _ptr(cache), pages, page, _ptr(tables),
+                                                   tables.shape[1], _ptr(lens), _ptr(row0), lens.numel(), q.shape[0], heads,
+                                                   n_kv, hd, window, sinks, scale, _ptr(out)))
 
     def dequantize(self, w: Weight, out):
         self._check(lib().hd_dequantize(self.h, w.h, _ptr(out), out.numel()))

@@ -2,7 +2,8 @@
  * hacedle_cuda.h -- C ABI of libhacedle_cuda.so, the B200 (sm_100a) kernels for
  * the quantized-weight hot path of the hacedle crate: GGUF block dequantization
  * (Q8_0, Q5_0, Q4_K, Q6_K) fused into GEMV / GEMM, plus the RMSNorm, RoPE,
- * GQA attention, SwiGLU and argmax kernels of a Qwen2-shaped decoder.
+ * GQA attention, SwiGLU and argmax kernels of a Qwen2-shaped decoder, and the
+ * page tables, 4-bit KV cache and sampler of a server around it.
  *
  * Conventions
  *  - Every function returns an hd_status (0 = HD_OK).  hd_last_error() gives
@@ -360,6 +361,26 @@ int hd_logits_process(hd_ctx *ctx, float *logits_dev, int64_t rows, int64_t n, f
 int hd_sample_rows(hd_ctx *ctx, const float *logits_dev, int64_t rows, int64_t n, uint64_t seed,
                    uint64_t offset, int32_t *idx_dev);
 
+/* One index per row from given random numbers u_dev [rows] in [0, 1), after the
+ * usual filters (hd_logits_process has the reference's own definitions).  With
+ * w_i = exp((x_i - max x) / T) in 64 bits, each row's own settings, and a NULL
+ * array turning its filter off (temperature: 1):
+ *   temperature_dev  T; T <= 0 or NaN: the first index of the maximum
+ *   top_k_dev        the k largest logits stay, of equal ones the lowest
+ *                    indices; k <= 0 or k >= n: all
+ *   top_p_dev        of those, in descending order (equal ones: lowest index
+ *                    first), the shortest prefix holding at least p of their
+ *                    mass; p >= 1 or NaN: all; p <= 0: one
+ *   min_p_dev        of those, the ones with w_i >= min_p (at most 1)
+ * and the draw is the first index, in the vocabulary's order, whose running
+ * sum of kept weights exceeds u times their sum (u outside [0, 1) is taken as
+ * the nearest inside).  NaN logits count as -infinity, which is never drawn; a
+ * row with nothing else gives -1.  ld: row stride of logits_dev in floats (0:
+ * n).  n < 2^31.  Sums are exact, so a draw depends on its inputs alone. */
+int hd_sample_filtered(hd_ctx *ctx, const float *logits_dev, int64_t ld, int64_t rows, int64_t n,
+                       const float *temperature_dev, const int32_t *top_k_dev, const float *top_p_dev,
+                       const float *min_p_dev, const float *u_dev, int32_t *idx_dev);
+
 /* -------------------------------------------------------- KV-cache arena */
 /* The device KV-cache manager (runtime/kv_cache.rs: KvArena :8-34, SessionKv
  * :37-56, SoulKv / SoulMemoryRegistry :58-118, KvCacheManager :121-127).
@@ -408,6 +429,91 @@ int hd_kv_append_slots(hd_ctx *ctx, const float *k_dev, const float *v_dev, floa
 int hd_attention_decode_slots(hd_ctx *ctx, const float *q_dev, const float *kc_dev, const float *vc_dev,
                               const int32_t *slots_dev, const int32_t *len_dev, int rows, int n_heads, int n_kv,
                               int head_dim, int max_ctx, float *out_dev);
+
+/* --------------------------------------------------------- paged KV cache */
+/* Serving many requests from one pool of pages.  The reference plans one slot
+ * per session (runtime/kv_cache.rs:8-34); these have no counterpart there.
+ * A page is page_size consecutive positions (a power of two, 16..1024) of one
+ * request; tables_dev [reqs][max_pages] int32 names request r's pages in
+ * order; a row's slot is page * page_size + position % page_size.
+ *
+ * hd_kv_pages_assign places new_dev[r] more tokens of each request behind its
+ * lens_dev[r] cached ones.  Pages that are needed beyond the
+ * ceil(len / page_size) held ones are taken from the end of the stack
+ * free_dev [*n_free_dev] in request order and written into the tables.
+ *   row0_dev [reqs + 1]   request r's new tokens are rows row0[r] .. row0[r+1]-1
+ *   slots_dev, pos_dev [max_rows]  each row's slot and position; -1 behind the
+ *                         last row (and the slot of a page id outside [0, pages))
+ *   lens_out_dev [reqs], n_free_out_dev [1]  the state after the step; they may
+ *                         be lens_dev and n_free_dev themselves
+ *   status_dev [1]        0; 1: the free pages do not suffice; 2: a length or
+ *                         count is negative or beyond max_pages * page_size;
+ *                         3: more than max_rows rows.  With 1..3 nothing is
+ *                         placed: tables, lengths and the free count stay, row0
+ *                         is all 0 and every slot -1.
+ * Up to 8192 requests.  free_dev must hold *n_free_dev ids. */
+int hd_kv_pages_assign(hd_ctx *ctx, const int32_t *lens_dev, const int32_t *new_dev, int reqs, int32_t *tables_dev,
+                       int max_pages, int page_size, int pages, const int32_t *free_dev, const int32_t *n_free_dev,
+                       int32_t *n_free_out_dev, int32_t *lens_out_dev, int32_t *row0_dev, int32_t *slots_dev,
+                       int32_t *pos_dev, int64_t max_rows, int32_t *status_dev);
+/* Returns the pages of every request with done_dev[r] != 0 to the end of the
+ * free stack (request order, table order), sets its length to 0 and its table
+ * entries to -1.  free_cap: ids free_dev has room for.  status_dev: 0; 1: they
+ * would not fit; 2: a length is out of range; with 1 and 2 nothing changes. */
+int hd_kv_pages_release(hd_ctx *ctx, const int32_t *done_dev, int32_t *lens_dev, int reqs, int32_t *tables_dev,
+                        int max_pages, int page_size, int32_t *free_dev, int32_t *n_free_dev, int free_cap,
+                        int32_t *status_dev);
+
+/* A layer's paged KV cache held in 4 bits: 4.5 bits a value, 7.1 times as many
+ * positions per byte as f32.  cache_dev (16-byte aligned, hd_kv4_cache_bytes)
+ * is [pages][n_kv][page_size / 16] tiles of 18 * head_dim bytes, each 16
+ * positions of one kv head:
+ *   K quants [16][head_dim / 2] | V quants [16][head_dim / 2]
+ *   | K scales f16 [16][head_dim / 32] | V scales f16 [16][head_dim / 32]
+ * with byte j of a group of 32 values holding value j in its low and value
+ * j + 16 in its high nibble (the GGUF order).  value = (nibble - 8) * d;
+ * d = f16(bf16(-x / 8) clamped to +-8160) for the group's first value x of
+ * largest magnitude, nibble = clamp(round-half-even(value / d) + 8, 0, 15).
+ * A group with a NaN reads back as NaN; infinities saturate.
+ * head_dim 32, 64 or 128; pages * page_size < 2^31. */
+uint64_t hd_kv4_cache_bytes(int64_t pages, int page_size, int n_kv, int head_dim);
+/* Row r's keys and values [n_kv][head_dim] (row strides k_ld, v_ld in floats;
+ * 0: n_kv * head_dim; rows 16-byte aligned) into slot slots_dev[r]; rows whose
+ * slot is outside [0, pages * page_size) are skipped.  The slots of one call
+ * must differ: what two rows leave in the same slot is not defined. */
+int hd_kv4_append(hd_ctx *ctx, const float *k_dev, const float *v_dev, int64_t k_ld, int64_t v_ld,
+                  const int32_t *slots_dev, int64_t rows, int n_kv, int head_dim, uint8_t *cache_dev, int64_t pages,
+                  int page_size);
+/* The values that slots hold, as f32 k_dev, v_dev [rows][n_kv][head_dim];
+ * zeros for a slot outside the cache. */
+int hd_kv4_read(hd_ctx *ctx, const uint8_t *cache_dev, int64_t pages, int page_size, const int32_t *slots_dev,
+                int64_t rows, int n_kv, int head_dim, float *k_dev, float *v_dev);
+/* GQA attention over the 4-bit cache (block.rs:138-173 with kv head =
+ * h / (n_heads / n_kv), at most 16 heads per kv head).  A query at position i
+ * sees position j <= i when window == 0 or j > i - window or j < sinks: a
+ * sliding window of the last `window` positions (itself among them) and
+ * `sinks` first ones that stay visible.  Positions on a table entry outside
+ * [0, pages) are not seen; a query that sees nothing gives zeros.  scale: of
+ * q . k; 0 means 1 / sqrt(head_dim).  q rows [n_heads][head_dim] with stride
+ * q_ld floats (0: dense; 16-byte aligned); out dense.  f32 accuracy: the
+ * cache's values enter exactly, q and the softmax weights in two f16 parts.
+ * decode:  row r is request r's last position, lens_dev[r] - 1.
+ *          ws_dev: hd_kv4_workspace_bytes bytes, zeroed once before their first
+ *          use, for calls that share nothing else in flight; NULL: the
+ *          context's own (two graphs that may replay at the same time need one
+ *          workspace each).
+ * prefill: rows row0[r] .. row0[r+1]-1 are the last positions of request r
+ *          (row0_dev [seqs + 1] ascending from 0); rows: of q and out; those
+ *          from row0[seqs] on are left as they are. */
+uint64_t hd_kv4_workspace_bytes(const hd_ctx *ctx, int n_heads, int n_kv, int head_dim);
+int hd_kv4_attention_decode(hd_ctx *ctx, const float *q_dev, int64_t q_ld, const uint8_t *cache_dev, int64_t pages,
+                            int page_size, const int32_t *tables_dev, int max_pages, const int32_t *lens_dev, int seqs,
+                            int n_heads, int n_kv, int head_dim, int window, int sinks, float scale, float *out_dev,
+                            void *ws_dev, size_t ws_bytes);
+int hd_kv4_attention_prefill(hd_ctx *ctx, const float *q_dev, int64_t q_ld, const uint8_t *cache_dev, int64_t pages,
+                             int page_size, const int32_t *tables_dev, int max_pages, const int32_t *lens_dev,
+                             const int32_t *row0_dev, int seqs, int64_t rows, int n_heads, int n_kv, int head_dim,
+                             int window, int sinks, float scale, float *out_dev);
 
 /* ------------------------------------------------------------ GGUF reader */
 /* Replaces GgufLoader::load_std, GgufTensorIndex::parse and tensor_bytes
