@@ -74,6 +74,7 @@ extern "C" int hd_ctx_destroy(hd_ctx *ctx) {
     cudaFree(ctx->kt_x);
     cudaFree(ctx->kt_y);
     cudaFree(ctx->amax_keys);
+    cudaFree(ctx->kv4_ws);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
     delete ctx;
     return HD_OK;

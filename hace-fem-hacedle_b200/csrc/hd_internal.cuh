@@ -60,6 +60,7 @@ struct hd_ctx {
     size_t samp_bytes = 0;
     float *kt_x = nullptr, *kt_y = nullptr;   // token-major copies for the [K][T] Q-GEMM entry points
     size_t kt_x_bytes = 0, kt_y_bytes = 0;
+    uint8_t *kv4_ws = nullptr;       // decode attention over the 4-bit cache: tickets (kept zero) and partials
     unsigned long long *amax_keys = nullptr;  // fused LM-head argmax: 16 keys + a CTA counter, kept zero
 };
 

@@ -11,26 +11,9 @@
 
 #include "hd_internal.cuh"
 #include "hd_kv4.cuh"
+#include "hd_kv4_args.cuh"
 
 namespace {
-
-constexpr int MAXREP4 = 16;
-
-struct Kv4Args {
-    const float *q;
-    int64_t q_ld;
-    const uint8_t *cache;
-    int64_t pages;
-    int shift;
-    const int32_t *tables;
-    int max_pages;
-    const int32_t *lens, *row0;   // row0: prefill; null: row r is request r's last position
-    int seqs;
-    int64_t rows;
-    int n_heads, n_kv, window, sinks;
-    float scale;
-    float *out;
-};
 
 // One CTA per query row and head, a warp per position.
 template <int HD>
@@ -118,7 +101,9 @@ int run(hd_ctx *ctx, const Kv4Args &A, int hd, const char *name) {
     return HD_OK;
 }
 
-int check(hd_ctx *ctx, const char *name, Kv4Args &A, int page_size, int hd) {
+}  // namespace
+
+int hd_kv4_attention_check(hd_ctx *ctx, const char *name, Kv4Args &A, int page_size, int hd) {
     if ((A.rows > 0 && (!A.q || !A.out)) || (A.seqs > 0 && (!A.tables || !A.lens)) || (A.pages > 0 && !A.cache))
         return hd_fail(ctx, HD_E_ARG, "%s: null argument", name);
     int rc = hd_kv4_check(ctx, name, A.cache, A.pages, page_size, A.n_kv, hd);
@@ -142,33 +127,13 @@ int check(hd_ctx *ctx, const char *name, Kv4Args &A, int page_size, int hd) {
     return HD_OK;
 }
 
-}  // namespace
-
-extern "C" uint64_t hd_kv4_workspace_bytes(const hd_ctx *ctx, int n_heads, int n_kv, int head_dim) {
-    return ctx && n_heads > 0 && n_kv > 0 && head_dim > 0 ? 256 : 0;
-}
-
-extern "C" int hd_kv4_attention_decode(hd_ctx *ctx, const float *q, int64_t q_ld, const uint8_t *cache, int64_t pages,
-                                       int page_size, const int32_t *tables, int max_pages, const int32_t *lens, int seqs,
-                                       int n_heads, int n_kv, int head_dim, int window, int sinks, float scale, float *out,
-                                       void *ws, size_t ws_bytes) {
-    Kv4Args A{q, q_ld, cache, pages, 0, tables, max_pages, lens, nullptr, seqs, seqs, n_heads, n_kv, window, sinks, scale, out};
-    int rc = check(ctx, "hd_kv4_attention_decode", A, page_size, head_dim);
-    if (rc || seqs == 0) return rc;
-    const uint64_t need = hd_kv4_workspace_bytes(ctx, n_heads, n_kv, head_dim);
-    HD_REQUIRE(ctx, !ws || ws_bytes >= need, HD_E_SHAPE, "hd_kv4_attention_decode: a workspace of %zu bytes (%llu needed)",
-               ws_bytes, (unsigned long long)need);
-    HdDevice on(ctx);
-    return run(ctx, A, head_dim, "hd_kv4_attention_decode");
-}
-
 extern "C" int hd_kv4_attention_prefill(hd_ctx *ctx, const float *q, int64_t q_ld, const uint8_t *cache, int64_t pages,
                                         int page_size, const int32_t *tables, int max_pages, const int32_t *lens,
                                         const int32_t *row0, int seqs, int64_t rows, int n_heads, int n_kv, int head_dim,
                                         int window, int sinks, float scale, float *out) {
     Kv4Args A{q, q_ld, cache, pages, 0, tables, max_pages, lens, row0, seqs, rows, n_heads, n_kv, window, sinks, scale, out};
     if (seqs > 0 && !row0) return hd_fail(ctx, HD_E_ARG, "hd_kv4_attention_prefill: null argument");
-    int rc = check(ctx, "hd_kv4_attention_prefill", A, page_size, head_dim);
+    int rc = hd_kv4_attention_check(ctx, "hd_kv4_attention_prefill", A, page_size, head_dim);
     if (rc || seqs == 0 || rows == 0) return rc;
     HdDevice on(ctx);
     return run(ctx, A, head_dim, "hd_kv4_attention_prefill");

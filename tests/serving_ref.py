@@ -78,7 +78,11 @@ def attention(q, k, v, ok, scale):
     the largest such error relative, plus 2^-21 for exp; and the output's sum
     of n terms in float32 by n / 4 + 64 roundings (partial sums of at least
     four parallel accumulators, then their merge) of 2^-24 of sum p |v|, for
-    the numerator and for the denominator."""
+    the numerator and for the denominator.  A weight enters its product in two
+    f16 parts after a scaling of the largest to 2^15; f16 has no bit below
+    2^-24, so besides its relative error each weight is off by up to half of
+    that, 2^-25 / 2^15 = 2^-40 of the largest weight, times its |v|: what a
+    dimension shows whose heavy positions all hold a zero."""
     heads, hd = q.shape
     rep = heads // k.shape[1]
     out, tol = np.zeros((heads, hd)), np.zeros((heads, hd))
@@ -91,7 +95,8 @@ def attention(q, k, v, ok, scale):
         p = np.exp(s - s.max())
         p /= p.sum()
         out[h] = p @ vv
-        tol[h] = (p @ np.abs(vv)) * (2 * ds + 2.0 ** -21 + 2 * (len(s) / 4 + 64) * 2.0 ** -24) + 1e-30
+        tol[h] = (p @ np.abs(vv)) * (2 * ds + 2.0 ** -21 + 2 * (len(s) / 4 + 64) * 2.0 ** -24) \
+            + 2.0 ** -40 * p.max() * np.abs(vv).sum(0)
     return out, tol
 
 

@@ -60,7 +60,9 @@ class Case:
 
 
 def _close(got, ref, tol):
-    assert np.all(np.abs(got - ref) <= tol), (np.abs(got - ref) / tol).max()
+    off = np.abs(got - ref)
+    at = np.unravel_index(np.argmax(off - tol), off.shape)
+    assert off[at] <= tol[at], (at, got[at], ref[at], tol[at])
 
 
 def _decode(ctx, torch, c, heads, window=0, sinks=0, scale=0.0, q=None, ws=None):
