@@ -34,20 +34,35 @@
 
 namespace {
 
-constexpr int DW = 4;           // warps per CTA
+#ifndef KV4_DW
+#define KV4_DW 4
+#endif
+constexpr int DW = KV4_DW;      // warps per CTA
 constexpr int DNT = 32 * DW;
-constexpr int DSTAGES = 5;      // tiles in a warp's ring
-constexpr int DMIN = 2 * DW;    // fewest tiles a CTA takes
-constexpr int DHEADS = 8;       // query heads per unit
-
+constexpr int DPT = 2;          // tiles per step
 template <int HD>
-constexpr int d_occ() { return HD == 128 ? 3 : 4; }   // CTAs per SM
+constexpr int d_stages() { return HD == 128 ? 2 : HD == 64 ? 3 : 4; }   // steps in a warp's ring
+constexpr int DMIN = DPT * DW;  // fewest tiles a CTA takes
+constexpr int DHEADS = 8;       // query heads per unit
+constexpr int DJOIN = 16;       // CTAs whose partials are joined first
+constexpr int DJOINS = 64;      // partials that one CTA joins at a time, at most
+
+#ifndef KV4_WARPS
+#define KV4_WARPS 16
+#endif
+template <int HD>
+constexpr int d_occ() { return KV4_WARPS / DW; }   // CTAs per SM
 
 template <int HD>
 struct DShared {
-    alignas(16) uint8_t ring[DW][DSTAGES][kv4_tile_bytes(HD)];
-    float o[DW][DHEADS][HD + 4];
+    union {
+        alignas(16) uint8_t ring[DW][d_stages<HD>()][DPT][kv4_tile_bytes(HD)];
+        alignas(16) float o[DW][DHEADS][HD + 4];      // the warps' outputs, once the ring is drained
+    };
+    alignas(16) uint32_t q[HD / 16][32][4];
     float m[DW][DHEADS], l[DW][DHEADS];
+    float ja[DJOINS * DHEADS], jl[DHEADS];
+    float kappa[DHEADS];
     int64_t part[DW];
     int64_t start_off;
     int start_req, last;
@@ -70,11 +85,43 @@ __device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
     __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
     return *reinterpret_cast<uint32_t *>(&r);
 }
-__device__ __forceinline__ uint32_t nib_lo(uint32_t w, uint32_t d2) {
-    return hmul2u(hsub2u((w & 0x000F000Fu) | H_MAGIC, 0x64086408u), d2);             // 1024 + n - 1032
+// `magic` is H_MAGIC from a register that the compiler cannot see through: as
+// a constant, mask and magic are two immediates and take two instructions.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+    return r;
 }
-__device__ __forceinline__ uint32_t nib_hi(uint32_t w, uint32_t d2) {
-    return hmul2u(hfma2u((w & 0x00F000F0u) | H_MAGIC, H_SIXTEENTH, 0xD480D480u), d2);  // (1024 + 16 n) / 16 - 72
+__device__ __forceinline__ uint32_t nib_lo(uint32_t w, uint32_t d2, uint32_t magic) {
+    return hmul2u(hsub2u(and_or(w, 0x000F000Fu, magic), 0x64086408u), d2);                // 1024 + n - 1032
+}
+__device__ __forceinline__ uint32_t nib_hi(uint32_t w, uint32_t d2, uint32_t magic) {
+    return hmul2u(hfma2u(and_or(w, 0x00F000F0u, magic), H_SIXTEENTH, 0xD480D480u), d2);   // (1024 + 16 n) / 16 - 72
+}
+
+// d += a b, m16n8k16, in place.
+__device__ __forceinline__ void mma_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Shared memory by its 32-bit address, in the order written (the rings are
+// filled behind the compiler's back).
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+    return v;
+}
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N]) {
+    static_assert(N == 1 || N == 2 || N == 4, "");
+    if constexpr (N == 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
+    else if constexpr (N == 2)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a));
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(a));
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -113,16 +160,105 @@ __device__ __forceinline__ Seen seen_tiles(const Kv4Args &A, int len) {
     return s;
 }
 
+// a / b, without the long division where 32 bits hold both.
+__device__ __forceinline__ int64_t div_fast(int64_t a, int64_t b) {
+    return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
+// A CTA's run may begin with the end of one item and end with the beginning
+// of another: two slots, the second for the item that begins in the run.
+__device__ __forceinline__ int slot_of(int cta, int first_cta) { return 2 * cta + (cta == first_cta ? 1 : 0); }
+
+// True in the CTA that arrives last of others + 1; the ticket is 0 again.
 template <int HD>
-__global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int groups, int gh, int *tickets, float *parts) {
+__device__ bool arrive(DShared<HD> &sm, int *ticket, int others) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sm.last = atomicAdd(ticket, 1) == others;
+        if (sm.last) *ticket = 0;
+    }
+    __syncthreads();
+    const bool last = sm.last;
+    __threadfence();
+    return last;
+}
+
+__device__ __forceinline__ void axpy4(float4 &y, float a, const float4 &x) {
+    y.x = fmaf(a, x.x, y.x);
+    y.y = fmaf(a, x.y, y.y);
+    y.z = fmaf(a, x.z, y.z);
+    y.w = fmaf(a, x.w, y.w);
+}
+__device__ __forceinline__ float4 over(const float4 &x, float l) {
+    return l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x / l, x.y / l, x.z / l, x.w / l);
+}
+
+// Joins n <= DJOINS partials, the i-th in slot slot_at(i), in order: into slot
+// `to` (a partial again; it may be one of them) or, for to < 0, the output.
+template <int HD, typename SlotAt>
+__device__ void join_parts(DShared<HD> &sm, float *parts, float2 *ml, int n, SlotAt slot_at, int nh, int to, float *out) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    // half a warp per head
+    for (int h = tid / 16; h < DHEADS; h += DNT / 16) {
+        float M = -INFINITY, L = 0.f;
+        for (int i = lane & 15; i < n; i += 16) M = fmaxf(M, __ldcg(ml + (int64_t)slot_at(i) * DHEADS + h).x);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float ref = M == -INFINITY ? 0.f : M;
+        for (int i = lane & 15; i < n; i += 16) {
+            const float2 v = __ldcg(ml + (int64_t)slot_at(i) * DHEADS + h);
+            const float a = exp2_approx(v.x - ref);
+            sm.ja[i * DHEADS + h] = a;
+            L = fmaf(v.y, a, L);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if ((lane & 15) == 0) {
+            sm.jl[h] = L;
+            if (to >= 0 && h < nh) sm.m[0][h] = M;
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < nh * (HD / 4); i += DNT) {
+        const int h = i / (HD / 4);
+        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int c = 0; c < n; c++)
+            axpy4(O, sm.ja[c * DHEADS + h], __ldcg((const float4 *)(parts + (int64_t)slot_at(c) * DHEADS * HD) + i));
+        if (to < 0) *((float4 *)out + i) = over(O, sm.jl[h]);
+        else __stcg((float4 *)(parts + (int64_t)to * DHEADS * HD) + i, O);   // each thread has read what it overwrites
+    }
+    if (to >= 0 && tid < nh) __stcg(ml + (int64_t)to * DHEADS + tid, make_float2(sm.m[0][tid], sm.jl[tid]));
+}
+
+template <int HD>
+__global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int groups, int gh, int *tickets, float2 *ml,
+                                                               float *parts) {
+    constexpr int NS = d_stages<HD>();
     constexpr int WPT = HD / 32;       // words of a key per thread
     constexpr int NT = HD / 8;         // column tiles of the output
-    constexpr int W = HD + 2;          // floats of a partial per head
     extern __shared__ __align__(16) uint8_t smem_raw[];
     DShared<HD> &sm = *reinterpret_cast<DShared<HD> *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     pdl_wait();
     pdl_trigger();
+    // this lane's place in a tile's copy: 16-byte piece `lane` of each 512 bytes, rows permuted
+    const uint32_t ring0 = smem_u32(sm.ring[warp][0][0]);
+    constexpr int PR = HD / 32;
+    const int my_slot = (lane / PR & 8) | d_slot<HD>(lane / PR & 7);
+    const uint32_t my_dst = HD == 32 ? 16u * lane : 16u * (my_slot * PR + d_piece<HD>(my_slot, lane % PR));
+    // where this lane reads a tile (first column tile of a step, first half of the positions)
+    const int kp = (g >> 1) + 4 * (g & 1), kslot = d_slot<HD>(kp);
+    constexpr int ROW = HD / 2;                     // bytes of a row's quants
+    const uint32_t k_at = kslot * ROW + (HD == 128 ? 16 * d_piece<HD>(kslot, t) : t * (HD / 8));
+    const uint32_t kd_at = 16 * HD + 2 * (kp * (HD / 32) + t * (HD / 8) / 16);
+    const int vslot = d_slot<HD>(t), vslot4 = d_slot<HD>(t + 4);
+    const uint32_t v_in = HD == 128 ? 16 * d_piece<HD>(vslot, g >> 1) + 8 * (g & 1) : g * (HD / 16);
+    const uint32_t v_at = 8 * HD + vslot * ROW + v_in, v4_at = 8 * HD + vslot4 * ROW + v_in;
+    const uint32_t vd_at = 17 * HD + 2 * (t * (HD / 32) + g * (HD / 16) / 16);
+    const uint32_t q_at = smem_u32(sm.q[0][lane]);
+    const uint32_t magic = H_MAGIC + (uint32_t)(A.shift >> 8);   // the shift is at most 10
     const int items = A.n_kv * groups, rep = A.n_heads / A.n_kv;
 
     // ---- this CTA's run of units
@@ -145,7 +281,7 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
     }
     total *= items;
     before *= items;
-    int64_t per = (total + gridDim.x - 1) / gridDim.x;
+    int64_t per = div_fast(total + gridDim.x - 1, gridDim.x);
     per = per < DMIN ? DMIN : per;
     const int64_t c_begin = per * blockIdx.x, c_end = min(total, c_begin + per);
     // requests without any position
@@ -174,42 +310,13 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
             req++;
             continue;
         }
-        const int item = (int)(off / S.units), u0 = (int)(off - (int64_t)item * S.units);
+        const int item = (int)div_fast(off, S.units), u0 = (int)(off - (int64_t)item * S.units);
         const int u1 = (int)min((int64_t)S.units, u0 + (c_end - at));
         const int kvh = item / groups, h0 = (item - kvh * groups) * gh, nh = min(gh, rep - h0);
         const int32_t *table = A.tables + (int64_t)req * A.max_pages;
 
-        // ---- tiles into the warp's ring
-        auto tile_of = [&](int u) { return u < S.sink ? u : S.from + u - S.sink; };
-        auto fetch = [&](int u, int stage) {
-            const int tile = tile_of(u), pos = tile * KV4_TILE;
-            const int64_t page = table[pos >> A.shift];
-            const bool ok = page >= 0 && page < A.pages;
-            if (ok) {
-                const uint8_t *src = A.cache + ((((page * A.n_kv + kvh) << A.shift) + (pos & ((1 << A.shift) - 1))) / KV4_TILE) *
-                                                   kv4_tile_bytes(HD);
-                const uint32_t dst = smem_u32(sm.ring[warp][stage]);
-                constexpr int PR = HD / 32, N = kv4_tile_bytes(HD) / 16;
-#pragma unroll
-                for (int i0 = 0; i0 < N; i0 += 32) {
-                    const int i = i0 + lane;
-                    if (i < N) {
-                        int to = i;
-                        if (i < 2 * 16 * PR) {           // quants: K rows 0..15, then V rows 0..15
-                            const int row = i / PR, slot = d_slot<HD>(row);
-                            to = slot * PR + d_piece<HD>(slot, i % PR);
-                        }
-                        cp16(dst + 16 * to, src + 16 * i);
-                    }
-                }
-            }
-            return ok;
-        };
-
-        // ---- q of the heads, in two f16 parts scaled to 2^14
-        uint32_t qa[WPT][2][4];
-        float kappa;                    // scores to base-2 exponents
-        {
+        // ---- q of the heads, in two f16 parts scaled to 2^14 (one warp; the others wait below)
+        if (warp == 0) {
             float x[WPT][8];
             const float *q = A.q + (int64_t)req * A.q_ld + (int64_t)(kvh * rep + h0 + g) * HD;
             float mx = 0.f;
@@ -233,84 +340,144 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
             int e = (int)(__float_as_uint(mx) >> 23) - 127;
             e = e < -100 ? -100 : e;
             const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-            kappa = A.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+            if (t == 0) sm.kappa[g] = A.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 #pragma unroll
             for (int w = 0; w < WPT; w++)
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
                     const float *v = x[w] + 4 * hf;
-                    split2(v[0] * up, v[2] * up, qa[w][hf][0], qa[w][hf][1]);
-                    split2(v[1] * up, v[3] * up, qa[w][hf][2], qa[w][hf][3]);
+                    uint4 f;
+                    split2(v[0] * up, v[2] * up, f.x, f.y);
+                    split2(v[1] * up, v[3] * up, f.z, f.w);
+                    *(uint4 *)sm.q[2 * w + hf][lane] = f;
                 }
         }
+
+        // ---- this warp's steps of two tiles: step k is units first_u + DPT * DW * k ..
+        const int first_u = u0 + DPT * warp;
+        const int n = u1 > first_u ? (u1 - first_u + DPT * DW - 1) / (DPT * DW) : 0;
+        // lane 2 i + j holds where tile j of step 16 * batch + i lies, or -1
+        auto look = [&](int batch) {
+            const int u = first_u + DPT * DW * (16 * batch + (lane >> 1)) + (lane & 1);
+            if (u >= u1) return -1;
+            const int tile = u < S.sink ? u : S.from + u - S.sink;
+            const int64_t page = table[tile >> (A.shift - 4)];
+            if (page < 0 || page >= A.pages) return -1;
+            return (int)(((page * A.n_kv + kvh) << (A.shift - 4)) + (tile & ((1 << (A.shift - 4)) - 1)));
+        };
+        int ids = look(0), ids_next = n > 16 ? look(1) : -1;
+        uint32_t named = 0;             // bits 2 s, 2 s + 1: the tiles of ring stage s exist
+        auto fetch = [&](int k, int stage) {
+            if (k < n) {
+                if (k && (k & 15) == 0) {
+                    ids = ids_next;
+                    ids_next = look(k / 16 + 1);
+                }
+#pragma unroll
+                for (int j = 0; j < DPT; j++) {
+                    const int at = __shfl_sync(0xffffffffu, ids, 2 * (k & 15) + j);
+                    named &= ~(1u << (DPT * stage + j));
+                    if (at < 0) continue;
+                    named |= 1u << (DPT * stage + j);
+                    const uint8_t *src = A.cache + (uint64_t)(uint32_t)at * kv4_tile_bytes(HD) + 16 * lane;
+                    const uint32_t dst = smem_u32(sm.ring[warp][stage][j]) + my_dst;
+                    constexpr int N = kv4_tile_bytes(HD) / 16, FULL = N / 32;
+#pragma unroll
+                    for (int c = 0; c < FULL; c++) cp16(dst + 512 * c, src + 512 * c);
+                    if (lane < N - 32 * FULL) cp16(ring0 + (uint32_t)(((stage * DPT) + j) * kv4_tile_bytes(HD)) + 512 * FULL + 16 * lane, src + 512 * FULL);
+                }
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < NS - 1; s++) fetch(s, s);
+        __syncthreads();                // q is there
+        const float kappa = sm.kappa[g];
         float o[NT][4], m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < NT; i++)
 #pragma unroll
             for (int c = 0; c < 4; c++) o[i][c] = 0.f;
 
-        uint32_t named = 0;             // bit s: the page of ring stage s exists
-        const int n = u1 - u0 > warp ? (u1 - u0 - warp + DW - 1) / DW : 0;   // this warp's tiles
-#pragma unroll
-        for (int s = 0; s < DSTAGES - 1; s++) {
-            if (s < n && fetch(u0 + warp + s * DW, s)) named |= 1u << s;
-            cp_commit();
-        }
+        // units whose 16 positions are all seen: from .. to - 1, and those below sinks
+        const int whole_from = S.sink + ((S.first & (KV4_TILE - 1)) != 0), whole_to = S.units - ((S.last + 1) % KV4_TILE != 0);
+        const int whole_sinks = min(A.sinks, S.first) / KV4_TILE;
         int stage = 0;
         for (int k = 0; k < n; k++) {
-            {
-                const int ahead = k + DSTAGES - 1, to = stage == 0 ? DSTAGES - 1 : stage - 1;
-                __syncwarp();           // all lanes have read the stage that is refilled
-                named &= ~(1u << to);
-                if (ahead < n && fetch(u0 + warp + ahead * DW, to)) named |= 1u << to;
-                cp_commit();
-            }
-            cp_wait<DSTAGES - 1>();
+            __syncwarp();               // all lanes have read the stage that is refilled
+            fetch(k + NS - 1, stage == 0 ? NS - 1 : stage - 1);
+            cp_wait<NS - 1>();
             __syncwarp();
-            const int pos = tile_of(u0 + warp + k * DW) * KV4_TILE;
-            const uint8_t *tile = sm.ring[warp][stage];
-            const bool ok = named >> stage & 1;
-            stage = stage == DSTAGES - 1 ? 0 : stage + 1;
+            const int u = first_u + DPT * DW * k;
+            const int cur = stage;
+            const uint32_t ok = named >> (DPT * stage) & 3;
+            stage = stage == NS - 1 ? 0 : stage + 1;
             if (!ok) continue;
-            const bool whole = pos + KV4_TILE - 1 <= S.last && (pos >= S.first || pos + KV4_TILE <= A.sinks);
-            auto sees = [&](int p) { return pos + p <= S.last && (pos + p >= S.first || pos + p < A.sinks); };
-
-            // ---- scores of positions t, t + 4 (first MMA) and t + 8, t + 12 (second)
-            float s[2][4];
+            const bool whole = ok == 3 && ((u >= whole_from && u + 1 < whole_to) || u + 1 < whole_sinks);
+            // a tile that is seen in part: the scales of the other positions become 0, so that whatever
+            // their slots hold counts for nothing (their scores are hidden below)
+            uint32_t hidden = 0;        // bit 16 j + p: position p of tile j is not seen
+            if (!whole) {
+                const int j = lane >> 4, p = lane & 15, uu = u + j;
+                const int at = (uu < S.sink ? uu : S.from + uu - S.sink) * KV4_TILE + p;
+                const bool sees = (ok >> j & 1) && at <= S.last && (at >= S.first || at < A.sinks);
+                if (!sees) {
+                    uint8_t *d = sm.ring[warp][cur][j] + 16 * HD + p * (HD / 16);
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int p = 8 * j + (g >> 1) + 4 * (g & 1), slot = d_slot<HD>(p);
-                uint32_t w[WPT];
-                const uint8_t *row = tile + slot * (HD / 2);
-                if constexpr (HD == 128) {
-                    const uint4 v = *(const uint4 *)(row + 16 * d_piece<HD>(slot, t));
-                    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-                } else if constexpr (HD == 64) {
-                    const uint2 v = *(const uint2 *)(row + 8 * t);
-                    w[0] = v.x; w[1] = v.y;
-                } else {
-                    w[0] = *(const uint32_t *)(row + 4 * t);
+                    for (int i = 0; i < HD / 32; i++) {
+                        *(uint16_t *)(d + 2 * i) = 0;
+                        *(uint16_t *)(d + HD + 2 * i) = 0;
+                    }
                 }
-                uint32_t d = *(const uint16_t *)(tile + 16 * HD + 2 * (p * (HD / 32) + t * (HD / 8) / 16));
-                if (!whole && !sees(p)) d = 0;
-                d |= d << 16;
+                hidden = __ballot_sync(0xffffffffu, !sees);
+                __syncwarp();
+            }
+
+            // ---- scores of positions t, t + 4 (first column tile) and t + 8, t + 12 (second) of each tile
+            const uint32_t base = ring0 + (uint32_t)(cur * DPT * kv4_tile_bytes(HD));
+            float s[2 * DPT][4];
+            uint32_t w[2 * DPT][WPT], dk[2 * DPT];
+#pragma unroll
+            for (int j = 0; j < 2 * DPT; j++) {
+                const uint32_t tile = base + (j >> 1) * kv4_tile_bytes(HD);
+                lds_words<WPT>(tile + k_at + (j & 1) * 8 * ROW, w[j]);
+                const uint32_t d = lds16(tile + kd_at + (j & 1) * (HD / 2));
+                dk[j] = __byte_perm(d, d, 0x1010);
 #pragma unroll
                 for (int c = 0; c < 4; c++) s[j][c] = 0.f;
+            }
 #pragma unroll
-                for (int i = 0; i < WPT; i++) {
-                    const uint32_t w8 = w[i] >> 8;
-                    mma16816(s[j], qa[i][0][0], qa[i][0][1], qa[i][0][2], qa[i][0][3], nib_lo(w[i], d), nib_lo(w8, d), s[j]);
-                    mma16816(s[j], qa[i][1][0], qa[i][1][1], qa[i][1][2], qa[i][1][3], nib_hi(w[i], d), nib_hi(w8, d), s[j]);
+            for (int i = 0; i < WPT; i++) {
+                uint32_t q0[4], q1[4];
+                lds_words<4>(q_at + 1024 * i, q0);
+                lds_words<4>(q_at + 1024 * i + 512, q1);
+#pragma unroll
+                for (int j = 0; j < 2 * DPT; j++) {
+                    const uint32_t w8 = w[j][i] >> 8;
+                    mma_add(s[j], q0[0], q0[1], q0[2], q0[3], nib_lo(w[j][i], dk[j], magic), nib_lo(w8, dk[j], magic));
+                    mma_add(s[j], q1[0], q1[1], q1[2], q1[3], nib_hi(w[j][i], dk[j], magic), nib_hi(w8, dk[j], magic));
                 }
             }
-            float e[4] = {(s[0][0] + s[0][2]) * kappa, (s[0][1] + s[0][3]) * kappa, (s[1][0] + s[1][2]) * kappa,
-                          (s[1][1] + s[1][3]) * kappa};
-            if (!whole) {
+            float e[DPT][4], mx = -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (!sees(t + 4 * c)) e[c] = -INFINITY;
+            for (int j = 0; j < DPT; j++) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    e[j][c] = (s[2 * j + (c >> 1)][c & 1] + s[2 * j + (c >> 1)][(c & 1) + 2]) * kappa;
+                }
             }
-            float mx = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3]));
+            if (hidden) {
+                const uint32_t mine_hidden = hidden >> t;
+#pragma unroll
+                for (int j = 0; j < DPT; j++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (mine_hidden >> (16 * j + 4 * c) & 1) e[j][c] = -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < DPT; j++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) mx = fmaxf(mx, e[j][c]);
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             if (__any_sync(0xffffffffu, mx > m)) {
@@ -323,64 +490,53 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
                     for (int c = 0; c < 4; c++) o[i][c] *= a;
             }
             const float ref = m == -INFINITY ? 0.f : m - 15.f;
+            uint32_t pa[DPT][4];
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                e[c] = exp2_approx(e[c] - ref);
-                l += e[c];
+            for (int j = 0; j < DPT; j++) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    e[j][c] = exp2_approx(e[j][c] - ref);
+                    l += e[j][c];
+                }
+                split2(e[j][0], e[j][1], pa[j][0], pa[j][1]);
+                split2(e[j][2], e[j][3], pa[j][2], pa[j][3]);
             }
-            uint32_t pa[4];
-            split2(e[0], e[1], pa[0], pa[1]);
-            split2(e[2], e[3], pa[2], pa[3]);
 
             // ---- output: value pairs (t, t + 4) and (t + 8, t + 12) of HD / 16 bytes of each row
-            constexpr int NX = HD >= 64 ? HD / 32 : 1;    // half words of a row's bytes
-            uint32_t x[2][NX], dd[2];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                uint32_t d[2];
-                if constexpr (HD == 32) {
-                    const int r0 = d_slot<HD>(8 * j + t), r1 = d_slot<HD>(8 * j + t + 4);
-                    const uint32_t a = *(const uint16_t *)(tile + 8 * HD + r0 * 16 + 2 * g);
-                    const uint32_t b = *(const uint16_t *)(tile + 8 * HD + r1 * 16 + 2 * g);
-                    x[j][0] = a | b << 16;
-                } else {
-                    uint32_t w[2][HD / 64];
+            for (int jt = 0; jt < DPT; jt++) {
+                const uint32_t tile = base + jt * kv4_tile_bytes(HD);
+                constexpr int NX = HD >= 64 ? HD / 32 : 1;    // half words of a row's bytes
+                uint32_t x[2][NX], dd[2];
 #pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        const int slot = d_slot<HD>(8 * j + t + 4 * y);
-                        const uint8_t *row = tile + 8 * HD + slot * (HD / 2);
-                        if constexpr (HD == 128) {
-                            const uint2 v = *(const uint2 *)(row + 16 * d_piece<HD>(slot, g >> 1) + 8 * (g & 1));
-                            w[y][0] = v.x;
-                            w[y][1] = v.y;
-                        } else {
-                            w[y][0] = *(const uint32_t *)(row + 4 * g);
+                for (int j = 0; j < 2; j++) {
+                    if constexpr (HD == 32) {
+                        x[j][0] = __byte_perm(lds16(tile + v_at + j * 8 * ROW), lds16(tile + v4_at + j * 8 * ROW), 0x5410);
+                    } else {
+                        uint32_t v0[HD / 64], v4[HD / 64];
+                        lds_words<HD / 64>(tile + v_at + j * 8 * ROW, v0);
+                        lds_words<HD / 64>(tile + v4_at + j * 8 * ROW, v4);
+#pragma unroll
+                        for (int i = 0; i < HD / 64; i++) {
+                            x[j][2 * i] = __byte_perm(v0[i], v4[i], 0x5410);
+                            x[j][2 * i + 1] = __byte_perm(v0[i], v4[i], 0x7632);
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < HD / 64; i++) {
-                        x[j][2 * i] = __byte_perm(w[0][i], w[1][i], 0x5410);
-                        x[j][2 * i + 1] = __byte_perm(w[0][i], w[1][i], 0x7632);
-                    }
+                    dd[j] = __byte_perm(lds16(tile + vd_at + j * (HD / 2)), lds16(tile + vd_at + HD / 4 + j * (HD / 2)), 0x5410);
                 }
+                const uint32_t(&pj)[4] = pa[jt];
 #pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    const int p = 8 * j + t + 4 * y;
-                    d[y] = *(const uint16_t *)(tile + 17 * HD + 2 * (p * (HD / 32) + g * (HD / 16) / 16));
-                    if (!whole && !sees(p)) d[y] = 0;
+                for (int i = 0; i < NX; i++) {
+                    const uint32_t y0 = x[0][i] >> 8, y1 = x[1][i] >> 8;
+                    mma_add(o[4 * i], pj[0], pj[1], pj[2], pj[3], nib_lo(x[0][i], dd[0], magic), nib_lo(x[1][i], dd[1], magic));
+                    mma_add(o[4 * i + 1], pj[0], pj[1], pj[2], pj[3], nib_hi(x[0][i], dd[0], magic), nib_hi(x[1][i], dd[1], magic));
+                    mma_add(o[4 * i + 2], pj[0], pj[1], pj[2], pj[3], nib_lo(y0, dd[0], magic), nib_lo(y1, dd[1], magic));
+                    mma_add(o[4 * i + 3], pj[0], pj[1], pj[2], pj[3], nib_hi(y0, dd[0], magic), nib_hi(y1, dd[1], magic));
                 }
-                dd[j] = d[0] | d[1] << 16;
-            }
-#pragma unroll
-            for (int i = 0; i < NX; i++) {
-                const uint32_t y0 = x[0][i] >> 8, y1 = x[1][i] >> 8;
-                mma16816(o[4 * i], pa[0], pa[1], pa[2], pa[3], nib_lo(x[0][i], dd[0]), nib_lo(x[1][i], dd[1]), o[4 * i]);
-                mma16816(o[4 * i + 1], pa[0], pa[1], pa[2], pa[3], nib_hi(x[0][i], dd[0]), nib_hi(x[1][i], dd[1]), o[4 * i + 1]);
-                mma16816(o[4 * i + 2], pa[0], pa[1], pa[2], pa[3], nib_lo(y0, dd[0]), nib_lo(y1, dd[1]), o[4 * i + 2]);
-                mma16816(o[4 * i + 3], pa[0], pa[1], pa[2], pa[3], nib_hi(y0, dd[0]), nib_hi(y1, dd[1]), o[4 * i + 3]);
             }
         }
         cp_wait<0>();
+        __syncthreads();                // every warp is done with the ring
 
         // ---- join the warps
         l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -400,55 +556,40 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
         const bool alone = u0 == 0 && u1 == S.units;
         // CTAs that share the item: from the one that holds its first unit
         const int64_t a0 = at - u0;
-        const int first_cta = (int)(a0 / per), last_cta = (int)((a0 + S.units - 1) / per);
-        float *mypart = parts + ((int64_t)blockIdx.x * 2 + (first_cta == (int)blockIdx.x ? 1 : 0)) * DHEADS * W;
+        const int first_cta = alone ? (int)blockIdx.x : (int)div_fast(a0, per), last_cta = alone ? (int)blockIdx.x : (int)div_fast(a0 + S.units - 1, per);
         float *out = A.out + ((int64_t)req * A.n_heads + kvh * rep + h0) * HD;
-        for (int i = tid; i < nh * HD; i += DNT) {
-            const int h = i / HD, d = i % HD;
+        const int slot = slot_of((int)blockIdx.x, first_cta);
+        for (int i = tid; i < nh * (HD / 4); i += DNT) {
+            const int h = i / (HD / 4), d = 4 * (i % (HD / 4));
             float M = -INFINITY;
 #pragma unroll
             for (int w = 0; w < DW; w++) M = fmaxf(M, sm.m[w][h]);
             const float ref = M == -INFINITY ? 0.f : M;
-            float O = 0.f, L = 0.f;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.f;
 #pragma unroll
             for (int w = 0; w < DW; w++) {
                 const float a = exp2_approx(sm.m[w][h] - ref);
-                O = fmaf(sm.o[w][h][d], a, O);
+                axpy4(O, a, *(const float4 *)&sm.o[w][h][d]);
                 L = fmaf(sm.l[w][h], a, L);
             }
             if (alone) {
-                out[i] = L == 0.f ? 0.f : O / L;
+                *((float4 *)out + i) = over(O, L);
             } else {
-                __stcg(mypart + h * W + d, O);
-                if (d == 0) {
-                    __stcg(mypart + h * W + HD, M);
-                    __stcg(mypart + h * W + HD + 1, L);
-                }
+                __stcg((float4 *)(parts + (int64_t)slot * DHEADS * HD) + i, O);
+                if (d == 0) __stcg(ml + (int64_t)slot * DHEADS + h, make_float2(M, L));
             }
         }
         if (!alone) {
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) sm.last = atomicAdd(tickets + first_cta, 1) == last_cta - first_cta;
-            __syncthreads();
-            if (sm.last) {
-                __threadfence();
-                for (int i = tid; i < nh * HD; i += DNT) {
-                    const int h = i / HD, d = i % HD;
-                    float M = -INFINITY, O = 0.f, L = 0.f;
-                    for (int c = first_cta; c <= last_cta; c++) {
-                        const float *p = parts + ((int64_t)c * 2 + (c == first_cta ? 1 : 0)) * DHEADS * W + h * W;
-                        const float pm = __ldcg(p + HD), mn = fmaxf(M, pm);
-                        if (__ldcg(p + HD + 1) != 0.f) {
-                            const float a = exp2_approx(M - mn), b = exp2_approx(pm - mn);
-                            O = O * a + __ldcg(p + d) * b;
-                            L = L * a + __ldcg(p + HD + 1) * b;
-                            M = mn;
-                        }
-                    }
-                    out[i] = L == 0.f ? 0.f : O / L;
-                }
-                if (tid == 0) tickets[first_cta] = 0;
+            // pieces join in aligned groups of DJOIN CTAs first, whose sums then join, each by whoever comes last
+            const int g0 = (int)blockIdx.x / DJOIN, gb = max(first_cta, g0 * DJOIN), ge = min(last_cta, g0 * DJOIN + DJOIN - 1);
+            const int f0 = first_cta / DJOIN, ng = last_cta / DJOIN - f0 + 1;
+            if (arrive(sm, tickets + slot_of(gb, first_cta), ge - gb)) {
+                join_parts<HD>(sm, parts, ml, ge - gb + 1, [&](int i) { return slot_of(gb + i, first_cta); }, nh,
+                               ng > 1 ? slot_of(gb, first_cta) : -1, out);
+                if (ng > 1 && arrive(sm, tickets + 2 * gridDim.x + first_cta, ng - 1))
+                    join_parts<HD>(sm, parts, ml, ng,
+                                   [&](int i) { return slot_of(max(first_cta, (f0 + i) * DJOIN), first_cta); }, nh, -1, out);
             }
         }
         __syncthreads();
@@ -458,7 +599,7 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
 }
 
 // CTAs of the largest grid.
-int max_ctas(const hd_ctx *ctx, int hd) { return ctx->sm_count * (hd == 128 ? d_occ<128>() : d_occ<64>()); }
+int max_ctas(const hd_ctx *ctx, int hd) { return min(ctx->sm_count * (hd == 128 ? d_occ<128>() : d_occ<64>()), DJOIN * DJOINS); }
 
 template <int HD>
 cudaError_t launch(hd_ctx *ctx, const Kv4Args &A, uint8_t *ws) {
@@ -472,11 +613,13 @@ cudaError_t launch(hd_ctx *ctx, const Kv4Args &A, uint8_t *ws) {
         const int64_t seen = ((int64_t)A.window + A.sinks) / KV4_TILE + 3;
         tiles = tiles < seen ? tiles : seen;
     }
-    const int64_t units = tiles * A.seqs * A.n_kv * groups, most = max_ctas(ctx, HD);
+    const int64_t units = tiles * A.seqs * A.n_kv * groups;
+    const int64_t most = max_ctas(ctx, HD);
     const int64_t want = (units + DMIN - 1) / DMIN;
     const int grid = (int)(want < most ? want : most);
-    return hd_launch(ctx, k_kv4_decode<HD>, dim3(grid), dim3(DNT), smem, A, groups, gh, (int *)ws,
-                     (float *)(ws + ((size_t)most * sizeof(int) + 255) / 256 * 256));
+    float2 *ml = (float2 *)(ws + ((size_t)3 * most * sizeof(int) + 255) / 256 * 256);
+    return hd_launch(ctx, k_kv4_decode<HD>, dim3(grid), dim3(DNT), smem, A, groups, gh, (int *)ws, ml,
+                     (float *)(ml + (size_t)2 * most * DHEADS));
 }
 
 }  // namespace
@@ -484,7 +627,7 @@ cudaError_t launch(hd_ctx *ctx, const Kv4Args &A, uint8_t *ws) {
 extern "C" uint64_t hd_kv4_workspace_bytes(const hd_ctx *ctx, int n_heads, int n_kv, int head_dim) {
     if (!ctx || n_heads <= 0 || n_kv <= 0 || (head_dim != 32 && head_dim != 64 && head_dim != 128)) return 0;
     const uint64_t g = (uint64_t)max_ctas(ctx, head_dim);
-    return (g * sizeof(int) + 255) / 256 * 256 + 2 * g * DHEADS * (head_dim + 2) * sizeof(float);
+    return (3 * g * sizeof(int) + 255) / 256 * 256 + 2 * g * DHEADS * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int hd_kv4_attention_decode(hd_ctx *ctx, const float *q, int64_t q_ld, const uint8_t *cache, int64_t pages,
