@@ -44,6 +44,7 @@ template <int HD>
 constexpr int d_stages() { return HD == 128 ? 2 : HD == 64 ? 3 : 4; }   // steps in a warp's ring
 constexpr int DMIN = DPT * DW;  // fewest tiles a CTA takes
 constexpr int DHEADS = 8;       // query heads per unit
+constexpr int DCOST = 16;       // what beginning an item costs, in tiles
 constexpr int DJOIN = 16;       // CTAs whose partials are joined first
 constexpr int DJOINS = 64;      // partials that one CTA joins at a time, at most
 
@@ -232,6 +233,10 @@ __device__ void join_parts(DShared<HD> &sm, float *parts, float2 *ml, int n, Slo
     if (to >= 0 && tid < nh) __stcg(ml + (int64_t)to * DHEADS + tid, make_float2(sm.m[0][tid], sm.jl[tid]));
 }
 
+// An item's length on the line that the CTAs share out: DCOST for its
+// beginning, then its tiles.
+__device__ __forceinline__ int cost_of(const Seen &s) { return s.units ? s.units + DCOST : 0; }
+
 template <int HD>
 __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int groups, int gh, int *tickets, float2 *ml,
                                                                float *parts) {
@@ -264,7 +269,7 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
     // ---- this CTA's run of units
     const int per_thread = (A.seqs + DNT - 1) / DNT, rb = min(A.seqs, tid * per_thread), re = min(A.seqs, rb + per_thread);
     int64_t mine = 0;
-    for (int r = rb; r < re; r++) mine += seen_tiles(A, A.lens[r]).units;
+    for (int r = rb; r < re; r++) mine += cost_of(seen_tiles(A, A.lens[r]));
     int64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -292,7 +297,7 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
     if (before <= c_begin && c_begin < before + mine * items) {
         int r = rb;
         for (;; r++) {
-            const int64_t u = (int64_t)seen_tiles(A, A.lens[r]).units * items;
+            const int64_t u = (int64_t)cost_of(seen_tiles(A, A.lens[r])) * items;
             if (c_begin < before + u) break;
             before += u;
         }
@@ -305,13 +310,19 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
 
     for (int64_t at = c_begin; at < c_end;) {
         const Seen S = seen_tiles(A, A.lens[req]);
-        if (off >= (int64_t)S.units * items) {
-            off -= (int64_t)S.units * items;
+        const int cost = cost_of(S);
+        if (off >= (int64_t)cost * items) {
+            off -= (int64_t)cost * items;
             req++;
             continue;
         }
-        const int item = (int)div_fast(off, S.units), u0 = (int)(off - (int64_t)item * S.units);
-        const int u1 = (int)min((int64_t)S.units, u0 + (c_end - at));
+        const int item = (int)div_fast(off, cost), o0 = (int)(off - (int64_t)item * cost);
+        const int o1 = (int)min((int64_t)cost, o0 + (c_end - at));
+        const int u0 = max(0, o0 - DCOST), u1 = max(0, o1 - DCOST);
+        const int64_t a0 = at - o0 + DCOST;         // where the item's tiles begin on the line
+        at += o1 - o0;
+        off += o1 - o0;
+        if (u0 >= u1) continue;
         const int kvh = item / groups, h0 = (item - kvh * groups) * gh, nh = min(gh, rep - h0);
         const int32_t *table = A.tables + (int64_t)req * A.max_pages;
 
@@ -555,7 +566,6 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
         __syncthreads();
         const bool alone = u0 == 0 && u1 == S.units;
         // CTAs that share the item: from the one that holds its first unit
-        const int64_t a0 = at - u0;
         const int first_cta = alone ? (int)blockIdx.x : (int)div_fast(a0, per), last_cta = alone ? (int)blockIdx.x : (int)div_fast(a0 + S.units - 1, per);
         float *out = A.out + ((int64_t)req * A.n_heads + kvh * rep + h0) * HD;
         const int slot = slot_of((int)blockIdx.x, first_cta);
@@ -593,8 +603,6 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
             }
         }
         __syncthreads();
-        at += u1 - u0;
-        off += u1 - u0;
     }
 }
 
@@ -613,9 +621,9 @@ cudaError_t launch(hd_ctx *ctx, const Kv4Args &A, uint8_t *ws) {
         const int64_t seen = ((int64_t)A.window + A.sinks) / KV4_TILE + 3;
         tiles = tiles < seen ? tiles : seen;
     }
-    const int64_t units = tiles * A.seqs * A.n_kv * groups;
+    const int64_t tiles_items = (int64_t)A.seqs * A.n_kv * groups, units = tiles * tiles_items;
     const int64_t most = max_ctas(ctx, HD);
-    const int64_t want = (units + DMIN - 1) / DMIN;
+    const int64_t want = (units + tiles_items * DCOST + DMIN - 1) / DMIN;
     const int grid = (int)(want < most ? want : most);
     float2 *ml = (float2 *)(ws + ((size_t)3 * most * sizeof(int) + 255) / 256 * 256);
     return hd_launch(ctx, k_kv4_decode<HD>, dim3(grid), dim3(DNT), smem, A, groups, gh, (int *)ws, ml,
