@@ -1,11 +1,11 @@
 """Filtered sampling against the 64-bit model: equal indices wherever no
 decision lies so close to its border that the weights' rounding could cross it.
 
-A weight is rounded to a multiple of 2^-s of the largest, s = 62 - ceil(log2 n),
-so it is off by at most 2^-(s+1), and the sums are exact; the n roundings are
-independent, each of standard deviation 2^-s / sqrt(12), so a running sum is
-off by 6 sqrt(n) 2^-s / sqrt(12) at six standard deviations, against a mass of
-at least 1.  The model's own sums in 64 bits add n 2^-53 of the mass at most."""
+A weight is rounded to a multiple of 2^-s of the largest, s = min(50, 62 -
+ceil(log2 n)), so it is off by at most 2^-(s+1), and the sums are exact; the n
+roundings are independent, each of standard deviation 2^-s / sqrt(12), so a
+running sum is off by 6 sqrt(n) 2^-s / sqrt(12) at six standard deviations,
+against a mass of at least 1; a weight itself is computed to 2^-48 of itself.  The model's own sums in 64 bits add n 2^-53 of the mass at most."""
 import numpy as np
 import pytest
 
@@ -29,7 +29,7 @@ def _run(ctx, torch, x, u, **kw):
 def _check(ctx, torch, x, u, temperature=None, top_k=None, top_p=None, min_p=None, on_border=1):
     """on_border: how many rows may lie on a border (rows of equal logits have whole masses that meet p exactly)."""
     n = x.shape[1]
-    near = 6 * np.sqrt(n / 12) * 2.0 ** (int(np.ceil(np.log2(n))) - 62) + n * 2.0 ** -53
+    near = 6 * np.sqrt(n / 12) * 2.0 ** max(-50, int(np.ceil(np.log2(n))) - 62) + 2.0 ** -48 + n * 2.0 ** -53
     got = _run(ctx, torch, x, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     at = lambda a, r, v: v if a is None else np.broadcast_to(a, (len(x),))[r]  # noqa: E731
     sure = 0
@@ -82,7 +82,7 @@ def test_rows_have_their_own_settings(ctx):
 def test_special_logits(ctx):
     import torch
     inf, nan = np.inf, np.nan
-    x = np.full((9, 777), -inf, np.float32)
+    x = np.full((9, 777), -inf, np.float32)   # (and rows of one CTA: the others span several)
     x[1, 700] = -3e38
     x[2, :] = nan
     x[3, [5, 9]] = nan, 2.0
@@ -157,3 +157,33 @@ def test_captured_and_replayed(ctx):
             assert idx.tolist() == want, step
     finally:
         ctx.set_stream(before)
+
+
+@pytest.mark.parametrize("n", [1_100_003, 5_000_000])
+def test_rows_beyond_shared_memory(ctx, n):
+    """A row that no cluster holds is read from memory at every step."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(2, n, generator=g, device="cuda") * 2
+    u = np.array([0.3, 0.8], np.float32)
+    for kw in ({"top_p": 0.9}, {"top_k": 500, "top_p": 0.7}, {"min_p": 0.001}):
+        got = _run(ctx, torch, x, u, **kw)
+        for r in range(2):
+            want, margin = R.sample(x[r].cpu().numpy(), u[r], k=kw.get("top_k", 0), p=kw.get("top_p", 1.0), min_p=kw.get("min_p", 0.0))
+            assert got[r] == want or margin < 1e-9
+
+
+def test_many_equal_logits_in_long_rows(ctx):
+    """The bin of the threshold holds more elements than are compared with one another, on several levels."""
+    import torch
+    rng = np.random.default_rng(31)
+    n = 100_000
+    x = np.empty((5, n), np.float32)
+    x[0] = 0.5                                                    # one key
+    x[1] = 1.0 + rng.integers(0, 3000, n).astype(np.float32) * np.float32(2.0 ** -23)   # 3000 neighbouring keys
+    x[2] = rng.standard_normal(n).astype(np.float32) * np.float32(1e-3)    # all in a few bins, keys far apart
+    x[3] = np.where(rng.random(n) < 0.5, 2.0, -1.0)
+    x[4] = np.where(np.arange(n) < n - 700, -40.0, 1.0)
+    u = rng.random(5).astype(np.float32)
+    for kw in ({"top_k": 33333}, {"top_p": 0.37}, {"top_k": 60001, "top_p": 0.61}, {"top_k": 99_999, "top_p": 0.999}):
+        _check(ctx, torch, x, u, on_border=3, **kw)
