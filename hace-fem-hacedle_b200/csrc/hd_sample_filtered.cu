@@ -12,21 +12,25 @@
 // All three filters keep a prefix of the descending order, so a row's kept
 // set is "key above tau, or one of the first c elements equal to tau", found
 // without a sort.  A row lies in the shared memory of a thread-block cluster
-// (read from memory once); a histogram over -log2 of the weight, 64 bins to a
-// factor of two, finds the bin in which the running count (top-k) or mass
-// (top-p) reaches its goal, and the few elements of that bin are compared with
-// one another.  More elements than CAP in a bin (many equal logits) are split
-// again by the bits of an order-preserving integer key.  Min-p is a smallest
-// key, found by search.  The draw adds up contiguous parts per CTA and per
-// warp and follows the target down.
+// (read from memory once).  A histogram of 64 bins over -log2 of the weight,
+// two to a factor of two, finds the bin in which the running count (top-k) or
+// mass (top-p) reaches its goal; that bin's elements are listed and split into
+// 1024 by the bits of an order-preserving integer key, and the few elements of
+// the one that is left are compared with one another (more than CAP of them --
+// many equal logits -- are split again).  Min-p is a smallest key, found by search.  The draw adds
+// up contiguous parts per CTA and per warp and follows the target down.
 //
-// Weights are computed in 64 bits (2^y = 2^(j/64) 2^e 2^r with a table of 64
-// and a polynomial of degree 5 in r, |r| <= 1/128: the table-driven method of
+// The first histogram has a copy per lane, a bank each: atomics on shared
+// memory were what bounded a single one (13 of 33 us per row, against 4 for
+// the weights), since logits crowd into few bins.
+//
+// Weights are computed in 64 bits (2^y = 2^(j/256) 2^e 2^r with a table of 256
+// and a polynomial of degree 4 in r, |r| <= 1/512: the table-driven method of
 // P. T. P. Tang, ACM TOMS 15 (1989), error below 2^-50) and held as whole
-// numbers of 2^-s, s = min(50, 62 - ceil(log2 n)): sums are exact in any order,
-// so neither atomics nor the shape of the cluster can change a draw, and a
-// weight's rounding (2^-45 of the largest for a vocabulary of 152k) is far
-// below what float32 sums lose.
+// numbers of 2^-s, s = 40 to 50 by the length of the row (42 for a vocabulary
+// of 152k): sums are exact in any order, so neither atomics nor the shape of
+// the cluster can change a draw, and a weight's rounding is far below what
+// float32 sums lose.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -37,32 +41,48 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int FBINS = 2048, FGROUP = 32, FGROUPS = FBINS / FGROUP;
+#ifndef FS_NT
+#define FS_NT 512
+#define FS_HALF 19456
+#define FS_OCC(NT) (1024 / NT)
+#endif
+constexpr int FBINS = 1024, FGROUP = 16, FGROUPS = FBINS / FGROUP;   // FGROUPS: also the first histogram's bins
+constexpr int CANDS = 2048;                  // elements of the first histogram's bin that a slice lists
 constexpr int CAP = 512;                     // elements compared with one another
 constexpr int MAXC = 16;                     // CTAs per row
 constexpr int MAXW = 32;                     // warps per CTA
 constexpr uint32_t KEY_NINF = 0x007fffffu;   // key of -infinity
 
-// Larger float, larger key; NaN counts as -infinity, -0 as 0.
+// Larger float, larger key (no NaN, no -0).
 __device__ __forceinline__ uint32_t order_key(float x) {
-    if (x != x) return KEY_NINF;
-    const uint32_t b = __float_as_uint(__fadd_rn(x, 0.f));
+    const uint32_t b = __float_as_uint(x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
+// NaN as -infinity, -0 as 0.
+__device__ __forceinline__ float plain(float v) { return v == v ? __fadd_rn(v, 0.f) : -INFINITY; }
+
 struct FShared {
-    uint32_t lo[FBINS], hi[FBINS];           // the slice's histogram, 64 bits in two halves
+    union {
+        struct {                             // the first histogram, a copy per lane; weights cut at Row::half bits
+            uint32_t lane_lo[FGROUPS * 32], lane_hi[FGROUPS * 32];
+        };
+        struct {                             // the others, 64 bits in two halves; the listed elements
+            uint32_t lo[FBINS], hi[FBINS], cand[CANDS];
+        };
+    };
+    long long part[MAXC][FGROUP];            // a group's bins of every CTA
     long long group[FGROUPS];                // its sums over groups of bins
     long long total[FGROUPS];                // the row's
-    double table[64];                        // 2^(j / 64)
+    double table[256];                       // 2^(j / 256), in units
     uint32_t list[CAP], all[CAP + 1];        // the slice's elements of a bin; the row's
     long long weight[CAP + 1];
     long long wsum[MAXW];                    // warps' sums
     int wtie[MAXW];
-    uint32_t n_list, kmax;                   // what other CTAs of the cluster read ..
+    uint32_t n_list, n_cand, kmax;           // what other CTAs of the cluster read ..
     long long mass;
     int ties;
     uint32_t pick;                           // .. and write
@@ -75,61 +95,69 @@ struct FShared {
 
 struct Row {
     const float *x;       // the slice
-    const uint4 *keys;    // its keys, where it is resident; padded with 0
+    const float4 *held;   // the same, where it is resident: NaN as -infinity, -0 as 0, and a NaN past the end
     int n, n4;            // its length; in fours
     double m, a;          // largest logit, log2(e) / temperature
-    uint32_t kmax;
-    int bits;             // units per weight 1: 2^bits
+    float top;            // m
+    bool inf;             // the largest is +infinity: read as 0, and all others as -infinity
+    int half;             // half the bits of a unit's weight 1
     const double *table;
+    __device__ __forceinline__ float seen(float v) const { return !inf || v != v ? v : v == INFINITY ? 0.f : -INFINITY; }
     template <bool RESIDENT>
-    __device__ __forceinline__ uint4 four(int i) const {
-        if (RESIDENT) return keys[i];
-        auto key = [&](int j) { return j < n ? order_key(x[j]) : 0u; };
-        return make_uint4(key(4 * i), key(4 * i + 1), key(4 * i + 2), key(4 * i + 3));
+    __device__ __forceinline__ float4 four(int i) const {
+        if (RESIDENT) return held[i];
+        auto one = [&](int j) { return j < n ? seen(plain(x[j])) : NAN; };
+        return make_float4(one(4 * i), one(4 * i + 1), one(4 * i + 2), one(4 * i + 3));
     }
     template <bool RESIDENT>
-    __device__ __forceinline__ uint32_t one(int i) const {
-        return RESIDENT ? ((const uint32_t *)keys)[i] : order_key(x[i]);
+    __device__ __forceinline__ float one(int i) const {
+        return RESIDENT ? ((const float *)held)[i] : seen(plain(x[i]));
     }
-    // log2 of the weight, rounded to a multiple of 1 / 64 (`k`: 1.5 * 2^46 above it)
-    __device__ __forceinline__ double log2w(uint32_t key, double &k) const {
-        const double y = ((double)key_value(key) - m) * a;
-        k = y + 0x1.8p46;
+    // y = log2 of the weight, <= 0, and k, whose low bits are 256 y rounded
+    __device__ __forceinline__ double log2w(float v, double &k) const {
+        const double y = ((double)v - m) * a;
+        k = y + 0x1.8p44;
         return y;
     }
-    // The bin of the first histogram: -64 log2(weight).
-    __device__ __forceinline__ static int bin(bool largest, double y, double k) {
-        return largest ? 0 : y >= -31.9 ? -__double2loint(k) : FBINS - 1;
+    // y < -64, where a weight is below half a unit (the high words of doubles <= 0 order as integers)
+    __device__ __forceinline__ static bool tiny(double y) { return (uint32_t)__double2hiint(y) >= 0xC0500000u; }
+    // The bin of the first histogram: -2 log2(weight).
+    __device__ __forceinline__ static int bin(bool tiny, double k) {
+        return tiny ? FGROUPS - 1 : min(-__double2loint(k) >> 7, FGROUPS - 1);
     }
-    __device__ __forceinline__ int bin(uint32_t key) const {
+    __device__ __forceinline__ int bin(float v) const {
         double k;
-        const double y = log2w(key, k);
-        return bin(key == kmax, y, k);
+        const double y = log2w(v, k);
+        return bin(tiny(y), k);
     }
-    __device__ __forceinline__ double weight(bool largest, double y, double k) const {
+    // The weight in units, as a double (not for tiny ones).
+    __device__ __forceinline__ double weight(double y, double k) const {
         const int ki = __double2loint(k);
-        const double r = y - (k - 0x1.8p46);
+        const double r = y - (k - 0x1.8p44);
         // 2^r - 1 = sum (r ln 2)^i / i!
-        double p = 0x1.5d87fe78a6730p-10;
-        p = fma(p, r, 0x1.3b2ab6fba4e77p-7);
+        double p = 0x1.3b2ab6fba4e77p-7;
         p = fma(p, r, 0x1.c6b08d704a0bfp-5);
         p = fma(p, r, 0x1.ebfbdff82c58ep-3);
         p = fma(p, r, 0x1.62e42fefa39efp-1);
         p *= r;
-        const double t = table[ki & 63], w = fma(t, p, t);
-        const double v = __hiloint2double(__double2hiint(w) + ((ki >> 6) << 20), __double2loint(w));
-        // below half a unit, or (-inf) * 0: nothing
-        return largest ? 1.0 : y >= -64.0 ? v : 0.0;
+        const double t = table[ki & 255], w = fma(t, p, t);
+        return __hiloint2double(__double2hiint(w) + ((ki >> 8) << 20), __double2loint(w));
     }
-    __device__ __forceinline__ double weight(uint32_t key) const {
+    __device__ __forceinline__ double weight(float v) const {
         double k;
-        const double y = log2w(key, k);
-        return weight(key == kmax, y, k);
+        const double y = log2w(v, k);
+        return tiny(y) ? 0.0 : weight(y, k);
     }
-    __device__ __forceinline__ long long units(double w) const {
-        // w 2^bits <= 2^50: adding 1.5 * 2^52 leaves the rounded integer in the low bits
-        const double v = w == 0.0 ? 0.0 : __hiloint2double(__double2hiint(w) + (bits << 20), __double2loint(w));
-        return __double_as_longlong(v + 0x1.8p52) - 0x4338000000000000ll;
+    // Rounded to whole units: at most 2^50 of them, so adding 1.5 * 2^52 leaves them in the low bits.
+    __device__ __forceinline__ static long long whole(double w) {
+        return __double_as_longlong(w + 0x1.8p52) - 0x4338000000000000ll;
+    }
+    // Branch-free, so that a thread's four elements interleave.
+    __device__ __forceinline__ long long units(float v) const {
+        double k;
+        const double y = log2w(v, k);
+        const long long w = whole(weight(y, k));
+        return tiny(y) ? 0 : w;
     }
 };
 
@@ -145,6 +173,13 @@ __device__ __forceinline__ long long warp_scan(long long v) {
         if ((int)(threadIdx.x & 31) >= o) v += x;
     }
     return v;
+}
+
+// 64 bits in two halves of 32, with the carry.
+__device__ __forceinline__ void add64(uint32_t *lo, uint32_t *hi, int b, unsigned long long w) {
+    const uint32_t wl = (uint32_t)w, old = atomicAdd(&lo[b], wl);
+    const uint32_t wh = (uint32_t)(w >> 32) + (old + wl < old ? 1u : 0u);
+    if (wh) atomicAdd(&hi[b], wh);
 }
 
 // f(rank) summed over the cluster, every load in flight at once.
@@ -191,59 +226,109 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned C = cluster.num_blocks(), rank = cluster.block_rank();
-    const long long floor_w = floor_ties > 0 ? floor_ties * (MASS ? R.units(R.weight(floor_key)) : 1) : 0;
-    uint32_t lo_key = floor_key + 1, hi_key = R.kmax;   // the elements in question; the floor's own come on top
+    const long long floor_w = floor_ties > 0 ? floor_ties * (MASS ? R.units(key_value(floor_key)) : 1) : 0;
+    uint32_t lo_key = max(floor_key + 1, KEY_NINF), hi_key = order_key(R.top);   // the elements in question; the floor's own come on top
     bool with_floor = floor_w > 0;
-    int shift = -1;                          // -1: bins of the weight; else of the key, from hi_key down
+    int shift = -1;                          // -1: the first histogram; else bins of the key, from hi_key down
+    long long own_above = 0;
     above = 0;
     own = -1;
     own_ties = 0;
-    for (;;) {
-        for (int b = tid; b < FBINS; b += NT) sm.lo[b] = sm.hi[b] = 0;
+    bool listed = false;                     // the elements in question are in every CTA's cand
+    // f(key) of each of them (and of the lanes' own pace; for few elements)
+    auto each = [&](auto f) {
+        if (listed) {
+            for (int i = tid; i < (int)sm.n_cand; i += NT) f(sm.cand[i]);
+        } else {
+            const float lo = key_value(lo_key), hi = key_value(hi_key);
+            auto in = [&](float v) { if (v >= lo && v <= hi) f(order_key(v)); };
+            for (int i = tid; i < R.n4; i += NT) {
+                const float4 v = R.four<RESIDENT>(i);
+                in(v.x);
+                in(v.y);
+                in(v.z);
+                in(v.w);
+            }
+        }
+    };
+    for (int level = 0;; level++) {
+        if (level == 0)
+            for (int b = tid; b < FGROUPS * 32; b += NT) sm.lane_lo[b] = sm.lane_hi[b] = 0;
+        else
+            for (int b = tid; b < FBINS; b += NT) sm.lo[b] = sm.hi[b] = 0;
         if (tid == 0) sm.n_list = 0;
         __syncthreads();
-        auto count = [&](uint32_t key) {
-            if (key < lo_key || key > hi_key) return;
-            double k, y;
-            int b;
-            if (shift < 0) {
-                y = R.log2w(key, k);
-                b = Row::bin(key == R.kmax, y, k);
-            } else {
-                b = (int)((hi_key - key) >> shift);
-                if (MASS) y = R.log2w(key, k);
+        if (level == 0) {
+            const uint32_t low = (1u << R.half) - 1;
+            const float least = key_value(lo_key);
+            auto count = [&](float v, double y, double k, unsigned long long w) {
+                const bool tiny = Row::tiny(y);
+                const int at = Row::bin(tiny, k) * 32 + lane;
+                if (!(v >= least)) return;
+                if (!MASS) {
+                    atomicAdd(&sm.lane_lo[at], 1u);
+                } else if (tiny) {
+                    return;
+                } else if (RESIDENT) {       // neither half can overflow, and no atomic returns anything
+                    atomicAdd(&sm.lane_lo[at], (uint32_t)w & low);
+                    atomicAdd(&sm.lane_hi[at], (uint32_t)(w >> R.half));
+                } else {
+                    add64(sm.lane_lo, sm.lane_hi, at, w);
+                }
+            };
+            for (int i = tid; i < R.n4; i += NT) {
+                const float4 v = R.four<RESIDENT>(i);
+                if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least)) continue;
+                double y[4], k[4];
+                unsigned long long w[4] = {0, 0, 0, 0};
+                y[0] = R.log2w(v.x, k[0]);
+                y[1] = R.log2w(v.y, k[1]);
+                y[2] = R.log2w(v.z, k[2]);
+                y[3] = R.log2w(v.w, k[3]);
+                if (MASS) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) w[c] = (unsigned long long)Row::whole(R.weight(y[c], k[c]));
+                }
+                count(v.x, y[0], k[0], w[0]);
+                count(v.y, y[1], k[1], w[1]);
+                count(v.z, y[2], k[2], w[2]);
+                count(v.w, y[3], k[3], w[3]);
             }
-            if (MASS) {
-                const unsigned long long w = (unsigned long long)R.units(R.weight(key == R.kmax, y, k));
-                const uint32_t wl = (uint32_t)w, old = atomicAdd(&sm.lo[b], wl);
-                const uint32_t wh = (uint32_t)(w >> 32) + (old + wl < old ? 1u : 0u);
-                if (wh) atomicAdd(&sm.hi[b], wh);
-            } else {
-                atomicAdd(&sm.lo[b], 1u);
-            }
-        };
-        for (int i = tid; i < R.n4; i += NT) {
-            const uint4 k = R.four<RESIDENT>(i);
-            count(k.x);
-            count(k.y);
-            count(k.z);
-            count(k.w);
+        } else {
+            auto count = [&](uint32_t key) {
+                if (key < lo_key || key > hi_key) return;
+                const int b = (int)((hi_key - key) >> shift);
+                if (!MASS) {
+                    atomicAdd(&sm.lo[b], 1u);
+                } else {
+                    add64(sm.lo, sm.hi, b, (unsigned long long)R.units(key_value(key)));
+                }
+            };
+            each(count);
         }
         __syncthreads();
-        // groups of 32 bins: eight threads a group
+        // groups of 16 bins, or the first histogram's bins of 32 lanes: eight threads each
         for (int q = tid / 8; q < FGROUPS; q += NT / 8) {
             unsigned long long s = 0;
+            if (level == 0) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int b = q * FGROUP + 4 * (tid & 7) + i;
-                s += ((unsigned long long)sm.hi[b] << 32) | sm.lo[b];
+                for (int i = 0; i < 4; i++) {
+                    const int b = q * 32 + 4 * (tid & 7) + i;
+                    s += ((unsigned long long)sm.lane_hi[b] << (RESIDENT ? R.half : 32)) + sm.lane_lo[b];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < FGROUP / 8; i++) {
+                    const int b = q * FGROUP + FGROUP / 8 * (tid & 7) + i;
+                    s += ((unsigned long long)sm.hi[b] << 32) + sm.lo[b];
+                }
             }
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
             if ((tid & 7) == 0) sm.group[q] = (long long)s;
         }
         cluster.sync();
-        const int floor_bin = !with_floor ? -1 : shift < 0 ? R.bin(floor_key) : (int)((hi_key - floor_key) >> shift);
+        const int floor_bin = !with_floor ? -1 : level == 0 ? R.bin(key_value(floor_key)) * FGROUP : (int)((hi_key - floor_key) >> shift);
         if (tid < FGROUPS)
             sm.total[tid] = (floor_bin >= 0 && floor_bin / FGROUP == tid ? floor_w : 0) +
                             cluster_sum(C, [&](unsigned r) { return cluster.map_shared_rank(&sm, r)->group[tid]; });
@@ -251,7 +336,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
         if (warp == 0) {
             const long long t0 = sm.total[2 * lane], t1 = sm.total[2 * lane + 1];
             const long long inc = warp_scan(t0 + t1);
-            if (MASS && shift < 0) {
+            if (MASS && level == 0) {
                 const long long mass = __shfl_sync(0xffffffffu, inc, 31);
                 goal = __double2ll_ru(p * (double)mass);
                 goal = goal < 1 ? 1 : goal > mass ? mass : goal;
@@ -261,29 +346,45 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
             const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
             const int q = __shfl_sync(0xffffffffu, b1 >= goal ? 2 * lane : 2 * lane + 1, src);
             const long long base = __shfl_sync(0xffffffffu, b1 >= goal ? b0 : b1, src);
-            const int b = q * FGROUP + lane;
-            const long long v = (floor_bin == b ? floor_w : 0) + cluster_sum(C, [&](unsigned r) {
-                                    const FShared *o = cluster.map_shared_rank(&sm, r);
-                                    return (long long)(((unsigned long long)o->hi[b] << 32) | o->lo[b]);
-                                });
-            const long long run = base + warp_scan(v);
-            const int first = __ffs(__ballot_sync(0xffffffffu, run >= goal)) - 1;
-            if (lane == first) {
-                sm.bin = b;
-                sm.bin_above = run - v;
+            if (lane == 0) {
+                sm.bin = q;
+                sm.bin_above = base;
+                sm.goal = goal;
             }
-            if (lane == 0) sm.goal = goal;
         }
         __syncthreads();
+        goal = sm.goal;
+        if (level > 0) {
+            // the group's bins: a warp per CTA fetches them, one adds them up
+            const int q = sm.bin;
+            if (warp < (int)C && lane < FGROUP) {
+                const FShared *o = cluster.map_shared_rank(&sm, warp);
+                sm.part[warp][lane] = (long long)(((unsigned long long)o->hi[q * FGROUP + lane] << 32) | o->lo[q * FGROUP + lane]);
+            }
+            __syncthreads();
+            if (warp == 0) {
+                const int b = q * FGROUP + lane;
+                long long v = lane < FGROUP && floor_bin == b ? floor_w : 0;
+                if (lane < FGROUP)
+                    for (unsigned r = 0; r < C; r++) v += sm.part[r][lane];
+                const long long run = sm.bin_above + warp_scan(v);
+                const int first = __ffs(__ballot_sync(0xffffffffu, run >= goal)) - 1;
+                __syncwarp();
+                if (lane == first) {
+                    sm.bin = b;
+                    sm.bin_above = run - v;
+                }
+            }
+            __syncthreads();
+        }
         const int pick = sm.bin;
         above = sm.bin_above;
-        goal = sm.goal;
         // the bin's keys
         uint32_t kl, kh;
-        if (shift < 0) {
+        if (level == 0) {
             if (warp < 2) {
                 const int v = pick + warp;   // the largest key of a bin >= v
-                const uint32_t k = v == 0 ? R.kmax : v >= FBINS ? KEY_NINF - 1 : last_key(R.kmax, [&](uint32_t c) { return R.bin(c) >= v; });
+                const uint32_t k = v == 0 ? order_key(R.top) : v >= FGROUPS ? KEY_NINF - 1 : last_key(order_key(R.top), [&](uint32_t c) { return R.bin(key_value(c)) >= v; });
                 if (lane == 0) sm.bound[warp] = k;
             }
             __syncthreads();
@@ -294,11 +395,59 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
             const uint32_t width = (1u << shift) - 1;
             kl = kh - lo_key < width ? lo_key : kh - width;
         }
-        if (floor_bin == pick) kl = floor_key;           // with the floor's own below the others
-        with_floor = floor_bin == pick;
+        with_floor = with_floor && (level == 0 ? floor_bin / FGROUP : floor_bin) == pick;
+        if (with_floor) kl = floor_key;      // the floor's own below the others
         if (kl == kh) {
             cluster.sync();                  // before the histogram is written again
             return kl;
+        }
+        if (level == 0) {
+            if (MASS)
+                for (int q = 0; q < pick; q++) own_above += sm.group[q];
+            lo_key = with_floor ? floor_key + 1 : kl;
+            hi_key = kh;
+            shift = 0;
+            while ((hi_key - kl) >> shift >= FBINS) shift++;
+            // list the bin's elements, over the histogram: its sums are in group, which nobody reads any more
+            // from here on but this CTA
+            if (tid == 0) sm.n_cand = 0;
+            __syncthreads();
+            const float lo = key_value(lo_key), hi = key_value(hi_key);
+            auto in = [&](float v) { return v >= lo && v <= hi; };
+            for (int i0 = 0; i0 < R.n4; i0 += NT) {
+                const float4 v = i0 + tid < R.n4 ? R.four<RESIDENT>(i0 + tid) : make_float4(NAN, NAN, NAN, NAN);
+                const int mine = (int)in(v.x) + in(v.y) + in(v.z) + in(v.w);
+                if (!__any_sync(0xffffffffu, mine)) continue;
+                int at = mine;               // a place for each lane's in the warp's run
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int x = __shfl_up_sync(0xffffffffu, at, o);
+                    if (lane >= o) at += x;
+                }
+                uint32_t base = 0;
+                if (lane == 31) base = atomicAdd(&sm.n_cand, (uint32_t)at);
+                uint32_t to = __shfl_sync(0xffffffffu, base, 31) + at - mine;
+                auto put = [&](float x) {
+                    if (in(x)) {
+                        if (to < CANDS) sm.cand[to] = order_key(x);
+                        to++;
+                    }
+                };
+                put(v.x);
+                put(v.y);
+                put(v.z);
+                put(v.w);
+            }
+            cluster.sync();
+            // by a warp, for all
+            if (warp == 0) {
+                const uint32_t c = cluster.map_shared_rank(&sm, lane < (int)C ? lane : 0)->n_cand;
+                const int ok = __all_sync(0xffffffffu, c <= CANDS);
+                if (lane == 0) sm.found = ok;
+            }
+            __syncthreads();
+            listed = sm.found;
+            continue;
         }
         const uint32_t kl_list = with_floor ? floor_key + 1 : kl;
         auto put = [&](uint32_t key) {
@@ -306,35 +455,30 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
             const uint32_t at = atomicAdd(&sm.n_list, 1u);
             if (at < CAP) sm.list[at] = key;
         };
-        for (int i = tid; i < R.n4; i += NT) {
-            const uint4 k = R.four<RESIDENT>(i);
-            put(k.x);
-            put(k.y);
-            put(k.z);
-            put(k.w);
-        }
+        each(put);
         cluster.sync();
-        uint32_t number[MAXC], all = 0;
+        // every warp learns the lists' lengths, a lane a CTA
+        const uint32_t number = lane < (int)C ? cluster.map_shared_rank(&sm, lane)->n_list : 0;
+        uint32_t upto = number;
 #pragma unroll
-        for (unsigned r = 0; r < MAXC; r++) number[r] = cluster.map_shared_rank(&sm, r < C ? r : 0)->n_list;
-#pragma unroll
-        for (unsigned r = 0; r < MAXC; r++) all += r < C ? number[r] : 0;
+        for (int o = 1; o < MAXC; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const uint32_t all = __shfl_sync(0xffffffffu, upto, MAXC - 1);
         if (all <= CAP) {
             // a warp per CTA's list
-            uint32_t start = 0;
-#pragma unroll
-            for (unsigned r = 0; r < MAXC; r++) {
-                if (r < C && (int)(r % NW) == warp) {
-                    const FShared *o = cluster.map_shared_rank(&sm, r);
-                    for (uint32_t i = lane; i < number[r]; i += 32) sm.all[start + i] = o->list[i];
-                }
-                start += r < C ? number[r] : 0;
+            const uint32_t len = __shfl_sync(0xffffffffu, number, warp & (MAXC - 1));
+            const uint32_t start = __shfl_sync(0xffffffffu, upto, warp & (MAXC - 1)) - len;
+            if (warp < (int)C) {
+                const FShared *o = cluster.map_shared_rank(&sm, warp);
+                for (uint32_t i = lane; i < len; i += 32) sm.all[start + i] = o->list[i];
             }
             if (with_floor && tid == 0) sm.all[all] = floor_key;
             const int L = (int)all + (with_floor ? 1 : 0);
             __syncthreads();
             for (int i = tid; i < L; i += NT)
-                sm.weight[i] = i == (int)all ? floor_w : MASS ? R.units(R.weight(sm.all[i])) : 1;
+                sm.weight[i] = i == (int)all ? floor_w : MASS ? R.units(key_value(sm.all[i])) : 1;
             __syncthreads();
             // every CTA compares its share of the elements with all of them, half a warp an element
             for (int i0 = (int)rank; i0 < L; i0 += (int)C * (NT / 16)) {
@@ -363,14 +507,14 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
             cluster.sync();                  // pick is there, and no list is read any more
             const uint32_t tau = sm.pick;
             above = sm.pick_above;
-            if (MASS && shift < 0) {
+            if (MASS && level == 1) {
                 // this slice above tau: its bins before the threshold's, and what the list adds
                 long long mass = 0;
                 for (int b = tid; b < pick; b += NT) mass += (long long)(((unsigned long long)sm.hi[b] << 32) | sm.lo[b]);
                 int tie = 0;
                 for (int i = tid; i < (int)sm.n_list; i += NT) {
                     const uint32_t key = sm.list[i];
-                    if (key > tau) mass += R.units(R.weight(key));
+                    if (key > tau) mass += R.units(key_value(key));
                     tie += key == tau;
                 }
                 mass = warp_sum(mass);
@@ -380,7 +524,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
                     sm.wtie[warp] = tie;
                 }
                 __syncthreads();
-                own = 0;
+                own = own_above;
                 for (int w = 0; w < NW; w++) {
                     own += sm.wsum[w];
                     own_ties += sm.wtie[w];
@@ -399,72 +543,80 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
 }
 
 template <int NT, bool RESIDENT>
-__global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *__restrict__ logits, int64_t ld, int64_t n,
+__global__ void __launch_bounds__(NT, FS_OCC(NT)) k_sample_filtered(const float *__restrict__ logits, int64_t ld, int64_t n,
                                                                    const float *__restrict__ temp,
                                                                    const int32_t *__restrict__ top_k,
                                                                    const float *__restrict__ top_p,
                                                                    const float *__restrict__ min_p,
-                                                                   const float *__restrict__ uni, int64_t slice, int bits,
+                                                                   const float *__restrict__ uni, int64_t slice, double unit, int half,
                                                                    int wide, int32_t *__restrict__ out) {
     constexpr int NW = NT / 32;
     extern __shared__ __align__(16) uint8_t raw[];
     FShared &sm = *reinterpret_cast<FShared *>(raw);
-    uint4 *keys = reinterpret_cast<uint4 *>(raw + (sizeof(FShared) + 15) / 16 * 16);
+    float4 *held = reinterpret_cast<float4 *>(raw + (sizeof(FShared) + 15) / 16 * 16);
     cg::cluster_group cluster = cg::this_cluster();
     const unsigned rank = cluster.block_rank(), C = cluster.num_blocks();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t r = blockIdx.x / C, begin = min(n, rank * slice), end = min(n, begin + slice);
     Row R;
     R.x = logits + r * ld + begin;
-    R.keys = keys;
+    R.held = held;
+    R.inf = false;
     R.n = (int)(end - begin);
     R.n4 = (R.n + 3) / 4;
-    if (tid < 64) sm.table[tid] = exp2((double)tid / 64);
+    for (int i = tid; i < 256; i += NT) sm.table[i] = exp2((double)i / 256) * unit;
     if (tid == 0) sm.kmax = 0;
     __syncthreads();
     pdl_wait();
     pdl_trigger();
-    uint32_t km = 0;
+    float mx = -INFINITY;
     const int whole = wide ? R.n / 4 : 0;    // 16-byte loads of an aligned row
 #pragma unroll 4
     for (int i = tid; i < whole; i += NT) {
         const float4 v = __ldcs((const float4 *)R.x + i);
-        const uint4 k = make_uint4(order_key(v.x), order_key(v.y), order_key(v.z), order_key(v.w));
-        km = max(max(km, max(k.x, k.y)), max(k.z, k.w));
-        if (RESIDENT) keys[i] = k;
+        const float4 q = make_float4(plain(v.x), plain(v.y), plain(v.z), plain(v.w));
+        mx = fmaxf(fmaxf(mx, fmaxf(q.x, q.y)), fmaxf(q.z, q.w));
+        if (RESIDENT) held[i] = q;
     }
 #pragma unroll 4
     for (int i = 4 * whole + tid; i < 4 * R.n4; i += NT) {
-        const uint32_t k = i < R.n ? order_key(R.x[i]) : 0;
-        km = max(km, k);
-        if (RESIDENT) ((uint32_t *)keys)[i] = k;
+        const float q = i < R.n ? plain(R.x[i]) : NAN;
+        mx = fmaxf(mx, q);
+        if (RESIDENT) ((float *)held)[i] = q;
     }
-    km = __reduce_max_sync(0xffffffffu, km);
+    const uint32_t km = __reduce_max_sync(0xffffffffu, order_key(mx));
     if (lane == 0) atomicMax(&sm.kmax, km);
     const float T = temp ? temp[r] : 1.f, u = uni[r];
     int64_t k = top_k ? top_k[r] : 0;
     float p = top_p ? top_p[r] : 1.f;
     double mp = min_p ? (double)min_p[r] : 0.0;
     cluster.sync();
-    R.kmax = 0;
-#pragma unroll
-    for (unsigned c = 0; c < MAXC; c++) R.kmax = max(R.kmax, cluster.map_shared_rank(&sm, c < C ? c : 0)->kmax);
+    const uint32_t kmax = __reduce_max_sync(0xffffffffu, cluster.map_shared_rank(&sm, lane < (int)C ? lane : 0)->kmax);
+    R.top = key_value(kmax);
     if (k <= 0 || k > n) k = n;
     if (p != p) p = 1.f;
     if (!(T > 0.f) || p <= 0.f) k = 1;
     mp = mp > 0.0 ? fmin(mp, 1.0) : 0.0;
-    R.m = (double)key_value(R.kmax);
-    R.a = 1.4426950408889634 / (double)T;
-    R.bits = bits;
+    if (R.top == INFINITY) {
+        R.inf = true;
+        R.top = 0.f;
+        if (RESIDENT) {
+            for (int i = tid; i < R.n4; i += NT) held[i] = make_float4(R.seen(held[i].x), R.seen(held[i].y), R.seen(held[i].z), R.seen(held[i].w));
+            __syncthreads();
+        }
+    }
+    R.m = (double)R.top;
+    R.a = T > 0.f ? fmax(1.4426950408889634 / (double)T, 1e-300) : 1.0;   // an infinite temperature leaves -infinity behind
+    R.half = half;
     R.table = sm.table;
     // tau, and how many of the elements equal to it stay
     uint32_t tau = 0;
     long long ties = 0, above, goal, own = -1;
     int own_ties = 0;
-    const bool none = R.kmax == KEY_NINF;
+    const bool none = kmax == KEY_NINF;
     if (!none) {
         if (k == 1) {
-            tau = R.kmax;
+            tau = order_key(R.top);
             ties = 1;
         } else {
             if (k < n) {
@@ -474,12 +626,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *
             }
             if (p < 1.f) {
                 tau = select<NT, RESIDENT, true>(R, sm, tau, ties, (double)p, goal, above, own, own_ties);
-                const long long w = R.units(R.weight(tau));
+                const long long w = R.units(key_value(tau));
                 ties = (goal - above + w - 1) / w;
             }
             if (mp > 0.0) {
                 // the smallest key with weight >= min_p
-                const uint32_t least = last_key(R.kmax, [&](uint32_t c) { return R.weight(c) < mp; }) + 1;
+                const uint32_t least = last_key(order_key(R.top), [&](uint32_t c) { return R.weight(key_value(c)) < mp * unit; }) + 1;
                 if (least > tau) {
                     tau = least;
                     ties = n;
@@ -489,23 +641,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *
         }
     }
     // ---- the draw
-    const long long wtau = tau ? R.units(R.weight(tau)) : 0;
+    const float ft = tau ? key_value(tau) : -INFINITY;   // (no filter: -infinity's weight is 0, kept or not)
+    const long long wtau = tau ? R.units(ft) : 0;
     auto part = [&](int b, int e) {          // a warp's fours b .. e - 1: their weight above tau, and ties
         long long mass = 0;
         int tie = 0;
-        auto add = [&](uint32_t key) {
-            if (key > tau) mass += R.units(R.weight(key));
-            tie += key == tau;
-        };
         for (int i = b + lane; i < e; i += 32) {
-            const uint4 q = R.four<RESIDENT>(i);
-            add(q.x);
-            add(q.y);
-            add(q.z);
-            add(q.w);
+            const float4 v = R.four<RESIDENT>(i);
+            tie += (int)(v.x == ft) + (int)(v.y == ft) + (int)(v.z == ft) + (int)(v.w == ft);
+            if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) > ft)) continue;
+            const long long w0 = R.units(v.x), w1 = R.units(v.y), w2 = R.units(v.z), w3 = R.units(v.w);
+            mass += (v.x > ft ? w0 : 0) + (v.y > ft ? w1 : 0) + (v.z > ft ? w2 : 0) + (v.w > ft ? w3 : 0);
         }
         mass = warp_sum(mass);
-        tie = __reduce_add_sync(0xffffffffu, tau ? tie : 0);
+        tie = __reduce_add_sync(0xffffffffu, tie);
         if (lane == 0) {
             sm.wsum[warp] = mass;
             sm.wtie[warp] = tie;
@@ -526,36 +675,31 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *
         sm.ties = tie;
     }
     cluster.sync();
-    // every CTA adds up the cluster; the one that holds the target goes on
-    long long masses[MAXC];
-    int tie_of[MAXC];
-#pragma unroll
-    for (unsigned c = 0; c < MAXC; c++) {
-        const FShared *o = cluster.map_shared_rank(&sm, c < C ? c : 0);
-        masses[c] = o->mass;
-        tie_of[c] = o->ties;
-    }
-    long long total = 0, mine = 0, my_mass = 0, tie_at = 0, my_tie = 0;
-#pragma unroll
-    for (unsigned c = 0; c < MAXC; c++) {
-        if (c >= C) continue;
-        if (c == rank) {
-            mine = total;
-            my_tie = tie_at;
+    // every CTA adds up the cluster, a lane a CTA; the one that holds the target goes on
+    if (warp == 0) {
+        const FShared *o = cluster.map_shared_rank(&sm, lane < (int)C ? lane : 0);
+        const long long mass = lane < (int)C ? o->mass : 0, tie = lane < (int)C ? o->ties : 0;
+        const long long t = warp_scan(tie) - tie;
+        const long long kept = mass + max(0ll, min(tie, ties - t)) * wtau, to = warp_scan(kept);
+        const long long total = __shfl_sync(0xffffffffu, to, 31);
+        long long target = (long long)((double)(u > 0.f ? u : 0.f) * (double)total);
+        target = target > total - 1 ? total - 1 : target;
+        if (lane == (int)rank) {
+            sm.found = to - kept <= target && target < to;
+            sm.goal = target;
+            sm.before = to - kept;
+            sm.tie_before = t;
         }
-        const long long kept = masses[c] + max(0ll, min((long long)tie_of[c], ties - tie_at)) * wtau;
-        if (c == rank) my_mass = kept;
-        total += kept;
-        tie_at += tie_of[c];
     }
     cluster.sync();                          // no CTA leaves while another reads it
     if (none) {
         if (rank == 0 && tid == 0) out[r] = -1;
         return;
     }
-    long long target = (long long)((double)(u > 0.f ? u : 0.f) * (double)total);
-    target = target > total - 1 ? total - 1 : target;
-    if (!(mine <= target && target < mine + my_mass)) return;
+    if (!sm.found) return;
+    const long long target = sm.goal;
+    long long mine = sm.before, my_tie = sm.tie_before;
+    __syncthreads();
     // from the slice to a warp's part of it, to a warp's part of that, to the element
     int b = 0, len = R.n4;
     for (int level = 0; level < 2; level++) {
@@ -584,11 +728,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *
     const int stop = min(R.n, 4 * (b + len));
     for (int i0 = 4 * b; i0 < stop; i0 += 32) {
         const int i = i0 + lane;
-        const uint32_t key = i < stop ? R.one<RESIDENT>(i) : 0;
-        const uint32_t eq = __ballot_sync(0xffffffffu, tau && key == tau);
+        const float v = i < stop ? R.one<RESIDENT>(i) : NAN;
+        const uint32_t eq = __ballot_sync(0xffffffffu, tau && v == ft);
         long long w = 0;
-        if (key > tau) w = R.units(R.weight(key));
-        else if (tau && key == tau && my_tie + __popc(eq & ((1u << lane) - 1u)) < ties) w = wtau;
+        if (v > ft) w = R.units(v);
+        else if (tau && v == ft && my_tie + __popc(eq & ((1u << lane) - 1u)) < ties) w = wtau;
         const long long run = mine + warp_scan(w);
         const uint32_t over = __ballot_sync(0xffffffffu, run > target);
         if (over) {
@@ -603,7 +747,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *
 template <int NT, bool RESIDENT>
 cudaError_t launch(hd_ctx *ctx, int C, int64_t rows, int64_t slice, const float *logits, int64_t ld, int64_t n,
                    const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p, const float *u,
-                   int bits, int32_t *idx) {
+                   double unit, int half, int32_t *idx) {
     const size_t smem = (sizeof(FShared) + 15) / 16 * 16 + (RESIDENT ? (size_t)slice * sizeof(float) : 0);
     auto kernel = k_sample_filtered<NT, RESIDENT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -611,7 +755,7 @@ cudaError_t launch(hd_ctx *ctx, int C, int64_t rows, int64_t slice, const float 
     if (e != cudaSuccess) return e;
     const int wide = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
     return hd_launch_cluster(ctx, kernel, dim3((unsigned)(rows * C)), dim3(NT), smem, C, logits, ld, n, temperature, top_k,
-                             top_p, min_p, u, slice, bits, wide, idx);
+                             top_p, min_p, u, slice, unit, half, wide, idx);
 }
 
 }  // namespace
@@ -627,19 +771,27 @@ extern "C" int hd_sample_filtered(hd_ctx *ctx, const float *logits, int64_t ld, 
     if (!ctx) return HD_E_ARG;
     if (rows == 0) return HD_OK;
     HdDevice on(ctx);
-    int bits = 0;
-    while (((int64_t)1 << bits) < n) bits++;
-    bits = 62 - bits < 50 ? 62 - bits : 50;
     // CTAs per row: as few as keep a slice at 80 KB, so that two CTAs share an SM; more while the rows
     // alone leave SMs idle and a slice keeps 2048 elements
-    constexpr int64_t HALF = 20480, FULL = 49152;
+    constexpr int64_t HALF = FS_HALF, FULL = 49152;
     auto slice_of = [&](int c) { return ((n + c - 1) / c + 3) / 4 * 4; };
     int C = 1;
     while (C < MAXC && (slice_of(C) > HALF || (rows * C < ctx->sm_count && slice_of(C) > 4096))) C *= 2;
     const int64_t slice = slice_of(C);
+    // Units: n of them sum below 2^62, and a lane's share of a resident slice times half of their bits below 2^32.
+    auto log2_up = [](int64_t v) {
+        int b = 0;
+        while (((int64_t)1 << b) < v) b++;
+        return b;
+    };
+    int bits = 62 - log2_up(n) < 50 ? 62 - log2_up(n) : 50;
+    const int room = 2 * (36 - log2_up(slice));
+    if (slice <= FULL && bits > room) bits = room;
+    const int half = (bits + 1) / 2;
+    const double unit = std::ldexp(1.0, bits);
     const bool few = rows * C <= ctx->sm_count;   // one CTA an SM: twice the threads
-#define HD_SAMPLE(NT, RES) launch<NT, RES>(ctx, C, rows, slice, logits, ld, n, temperature, top_k, top_p, min_p, u, bits, idx)
-    cudaError_t e = slice > FULL ? HD_SAMPLE(1024, false) : few ? HD_SAMPLE(1024, true) : HD_SAMPLE(512, true);
+#define HD_SAMPLE(NT, RES) launch<NT, RES>(ctx, C, rows, slice, logits, ld, n, temperature, top_k, top_p, min_p, u, unit, half, idx)
+    cudaError_t e = slice > FULL ? HD_SAMPLE(1024, false) : few ? HD_SAMPLE(1024, true) : HD_SAMPLE(FS_NT, true);
 #undef HD_SAMPLE
     if (e != cudaSuccess) return hd_fail(ctx, HD_E_CUDA, "hd_sample_filtered: %s", cudaGetErrorString(e));
     return HD_OK;

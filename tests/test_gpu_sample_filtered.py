@@ -1,10 +1,10 @@
 """Filtered sampling against the 64-bit model: equal indices wherever no
 decision lies so close to its border that the weights' rounding could cross it.
 
-A weight is rounded to a multiple of 2^-s of the largest, s = min(50, 62 -
-ceil(log2 n)), so it is off by at most 2^-(s+1), and the sums are exact; the n
-roundings are independent, each of standard deviation 2^-s / sqrt(12), so a
-running sum is off by 6 sqrt(n) 2^-s / sqrt(12) at six standard deviations,
+A weight is rounded to a multiple of 2^-s of the largest, s at least 40 (more
+for rows of less than 786432), so it is off by at most 2^-41, and the sums are
+exact; the n roundings are independent, each of standard deviation 2^-40 / sqrt(12), so a
+running sum is off by 6 sqrt(n) 2^-40 / sqrt(12) at six standard deviations,
 against a mass of at least 1; a weight itself is computed to 2^-48 of itself.  The model's own sums in 64 bits add n 2^-53 of the mass at most."""
 import numpy as np
 import pytest
@@ -29,7 +29,7 @@ def _run(ctx, torch, x, u, **kw):
 def _check(ctx, torch, x, u, temperature=None, top_k=None, top_p=None, min_p=None, on_border=1):
     """on_border: how many rows may lie on a border (rows of equal logits have whole masses that meet p exactly)."""
     n = x.shape[1]
-    near = 6 * np.sqrt(n / 12) * 2.0 ** max(-50, int(np.ceil(np.log2(n))) - 62) + 2.0 ** -48 + n * 2.0 ** -53
+    near = 6 * np.sqrt(n / 12) * 2.0 ** -40 + 2.0 ** -48 + n * 2.0 ** -53
     got = _run(ctx, torch, x, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     at = lambda a, r, v: v if a is None else np.broadcast_to(a, (len(x),))[r]  # noqa: E731
     sure = 0
@@ -54,7 +54,8 @@ def test_matches_the_model(ctx, rows, n, kw):
     import torch
     rng = np.random.default_rng(n + rows)
     x = (rng.standard_normal((rows, n)) * 2.5).astype(np.float32)
-    _check(ctx, torch, x, rng.random(rows).astype(np.float32), **kw)
+    # (at top_p = 0.99999 the running mass moves by about 1e-10 of itself per index of a long row: rows may lie on a border)
+    _check(ctx, torch, x, rng.random(rows).astype(np.float32), on_border=2 if kw.get("top_p") == 0.99999 and n > 100000 else 1, **kw)
 
 
 @pytest.mark.parametrize("kw", SETTINGS, ids=str)
