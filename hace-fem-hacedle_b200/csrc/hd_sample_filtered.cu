@@ -65,34 +65,6 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // NaN as -infinity, -0 as 0.
 __device__ __forceinline__ float plain(float v) { return v == v ? __fadd_rn(v, 0.f) : -INFINITY; }
 
-struct FShared {
-    union {
-        struct {                             // the first histogram, a copy per lane; weights cut at Row::half bits
-            uint32_t lane_lo[FGROUPS * 32], lane_hi[FGROUPS * 32];
-        };
-        struct {                             // the others, 64 bits in two halves; the listed elements
-            uint32_t lo[FBINS], hi[FBINS], cand[CANDS];
-        };
-    };
-    long long part[MAXC][FGROUP];            // a group's bins of every CTA
-    long long group[FGROUPS];                // its sums over groups of bins
-    long long total[FGROUPS];                // the row's
-    double table[256];                       // 2^(j / 256), in units
-    uint32_t list[CAP], all[CAP + 1];        // the slice's elements of a bin; the row's
-    long long weight[CAP + 1];
-    long long wsum[MAXW];                    // warps' sums
-    int wtie[MAXW];
-    uint32_t n_list, n_cand, kmax;           // what other CTAs of the cluster read ..
-    long long mass;
-    int ties;
-    uint32_t pick;                           // .. and write
-    long long pick_above;
-    int bin;                                 // broadcasts within the CTA
-    long long bin_above, goal, before, tie_before;
-    uint32_t bound[2];
-    int found;
-};
-
 struct Row {
     const float *x;       // the slice
     const float4 *held;   // the same, where it is resident: NaN as -infinity, -0 as 0, and a NaN past the end
@@ -161,6 +133,35 @@ struct Row {
     }
 };
 
+struct FShared {
+    union {
+        struct {                             // the first histogram, a copy per lane; weights cut at Row::half bits
+            uint32_t lane_lo[FGROUPS * 32], lane_hi[FGROUPS * 32];
+        };
+        struct {                             // the others, 64 bits in two halves; the listed elements
+            uint32_t lo[FBINS], hi[FBINS], cand[CANDS];
+        };
+    };
+    long long part[MAXC][FGROUP];            // a group's bins of every CTA
+    long long group[FGROUPS];                // its sums over groups of bins
+    long long total[FGROUPS];                // the row's
+    Row row;
+    double table[256];                       // 2^(j / 256), in units
+    uint32_t list[CAP], all[CAP + 1];        // the slice's elements of a bin; the row's
+    long long weight[CAP + 1];
+    long long wsum[MAXW];                    // warps' sums
+    int wtie[MAXW];
+    uint32_t n_list, n_cand, kmax;           // what other CTAs of the cluster read ..
+    long long mass;
+    int ties;
+    uint32_t pick;                           // .. and write
+    long long pick_above;
+    int bin;                                 // broadcasts within the CTA
+    long long bin_above, goal, before, tie_before;
+    uint32_t bound[2];
+    int found;
+};
+
 __device__ __forceinline__ long long warp_sum(long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -180,6 +181,104 @@ __device__ __forceinline__ void add64(uint32_t *lo, uint32_t *hi, int b, unsigne
     const uint32_t wl = (uint32_t)w, old = atomicAdd(&lo[b], wl);
     const uint32_t wh = (uint32_t)(w >> 32) + (old + wl < old ? 1u : 0u);
     if (wh) atomicAdd(&hi[b], wh);
+}
+
+// The loops over a slice are functions of their own: inlined, what the rest of
+// the kernel holds was spilled inside them (14 of 45 instructions an element).
+
+// Every element >= least into the first histogram: 1, or (MASS) its units.
+template <int NT, bool RESIDENT, bool MASS>
+__device__ __noinline__ void first_histogram(FShared &sm, float least) {
+    const Row R = sm.row;
+    const int tid = threadIdx.x, lane = tid & 31;
+                const uint32_t low = (1u << R.half) - 1;
+                auto count = [&](float v, double y, double k, unsigned long long w) {
+                    const bool tiny = Row::tiny(y);
+                    const int at = Row::bin(tiny, k) * 32 + lane;
+                    if (!(v >= least)) return;
+                    if (!MASS) {
+                        atomicAdd(&sm.lane_lo[at], 1u);
+                    } else if (tiny) {
+                        return;
+                    } else if (RESIDENT) {       // neither half can overflow, and no atomic returns anything
+                        atomicAdd(&sm.lane_lo[at], (uint32_t)w & low);
+                        atomicAdd(&sm.lane_hi[at], (uint32_t)(w >> R.half));
+                    } else {
+                        add64(sm.lane_lo, sm.lane_hi, at, w);
+                    }
+                };
+                for (int i = tid; i < R.n4; i += NT) {
+                    const float4 v = R.four<RESIDENT>(i);
+                    if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least)) continue;
+                    double y[4], k[4];
+                    unsigned long long w[4] = {0, 0, 0, 0};
+                    y[0] = R.log2w(v.x, k[0]);
+                    y[1] = R.log2w(v.y, k[1]);
+                    y[2] = R.log2w(v.z, k[2]);
+                    y[3] = R.log2w(v.w, k[3]);
+                    if (MASS) {
+    #pragma unroll
+                        for (int c = 0; c < 4; c++) w[c] = (unsigned long long)Row::whole(R.weight(y[c], k[c]));
+                    }
+                    count(v.x, y[0], k[0], w[0]);
+                    count(v.y, y[1], k[1], w[1]);
+                    count(v.z, y[2], k[2], w[2]);
+                    count(v.w, y[3], k[3], w[3]);
+                }
+}
+
+// The keys of the elements lo .. hi into cand, in any order.
+template <int NT, bool RESIDENT>
+__device__ __noinline__ void list_bin(FShared &sm, float lo, float hi) {
+    const Row R = sm.row;
+    const int tid = threadIdx.x, lane = tid & 31;
+                            auto in = [&](float v) { return v >= lo && v <= hi; };
+                for (int i0 = 0; i0 < R.n4; i0 += NT) {
+                    const float4 v = i0 + tid < R.n4 ? R.four<RESIDENT>(i0 + tid) : make_float4(NAN, NAN, NAN, NAN);
+                    const int mine = (int)in(v.x) + in(v.y) + in(v.z) + in(v.w);
+                    if (!__any_sync(0xffffffffu, mine)) continue;
+                    int at = mine;               // a place for each lane's in the warp's run
+    #pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int x = __shfl_up_sync(0xffffffffu, at, o);
+                        if (lane >= o) at += x;
+                    }
+                    uint32_t base = 0;
+                    if (lane == 31) base = atomicAdd(&sm.n_cand, (uint32_t)at);
+                    uint32_t to = __shfl_sync(0xffffffffu, base, 31) + at - mine;
+                    auto put = [&](float x) {
+                        if (in(x)) {
+                            if (to < CANDS) sm.cand[to] = order_key(x);
+                            to++;
+                        }
+                    };
+                    put(v.x);
+                    put(v.y);
+                    put(v.z);
+                    put(v.w);
+                }
+}
+
+// A warp's fours b .. e - 1: their weight above ft, and how many equal it.
+template <bool RESIDENT>
+__device__ __noinline__ void part(FShared &sm, int b, int e, float ft) {
+    const Row R = sm.row;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long mass = 0;
+    int tie = 0;
+    for (int i = b + lane; i < e; i += 32) {
+        const float4 v = R.four<RESIDENT>(i);
+        tie += (int)(v.x == ft) + (int)(v.y == ft) + (int)(v.z == ft) + (int)(v.w == ft);
+        if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) > ft)) continue;
+        const long long w0 = R.units(v.x), w1 = R.units(v.y), w2 = R.units(v.z), w3 = R.units(v.w);
+        mass += (v.x > ft ? w0 : 0) + (v.y > ft ? w1 : 0) + (v.z > ft ? w2 : 0) + (v.w > ft ? w3 : 0);
+    }
+    mass = warp_sum(mass);
+    tie = __reduce_add_sync(0xffffffffu, tie);
+    if (lane == 0) {
+        sm.wsum[warp] = mass;
+        sm.wtie[warp] = tie;
+    }
 }
 
 // f(rank) summed over the cluster, every load in flight at once.
@@ -259,41 +358,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
         if (tid == 0) sm.n_list = 0;
         __syncthreads();
         if (level == 0) {
-            const uint32_t low = (1u << R.half) - 1;
-            const float least = key_value(lo_key);
-            auto count = [&](float v, double y, double k, unsigned long long w) {
-                const bool tiny = Row::tiny(y);
-                const int at = Row::bin(tiny, k) * 32 + lane;
-                if (!(v >= least)) return;
-                if (!MASS) {
-                    atomicAdd(&sm.lane_lo[at], 1u);
-                } else if (tiny) {
-                    return;
-                } else if (RESIDENT) {       // neither half can overflow, and no atomic returns anything
-                    atomicAdd(&sm.lane_lo[at], (uint32_t)w & low);
-                    atomicAdd(&sm.lane_hi[at], (uint32_t)(w >> R.half));
-                } else {
-                    add64(sm.lane_lo, sm.lane_hi, at, w);
-                }
-            };
-            for (int i = tid; i < R.n4; i += NT) {
-                const float4 v = R.four<RESIDENT>(i);
-                if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least)) continue;
-                double y[4], k[4];
-                unsigned long long w[4] = {0, 0, 0, 0};
-                y[0] = R.log2w(v.x, k[0]);
-                y[1] = R.log2w(v.y, k[1]);
-                y[2] = R.log2w(v.z, k[2]);
-                y[3] = R.log2w(v.w, k[3]);
-                if (MASS) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++) w[c] = (unsigned long long)Row::whole(R.weight(y[c], k[c]));
-                }
-                count(v.x, y[0], k[0], w[0]);
-                count(v.y, y[1], k[1], w[1]);
-                count(v.z, y[2], k[2], w[2]);
-                count(v.w, y[3], k[3], w[3]);
-            }
+            first_histogram<NT, RESIDENT, MASS>(sm, key_value(lo_key));
         } else {
             auto count = [&](uint32_t key) {
                 if (key < lo_key || key > hi_key) return;
@@ -412,32 +477,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
             // from here on but this CTA
             if (tid == 0) sm.n_cand = 0;
             __syncthreads();
-            const float lo = key_value(lo_key), hi = key_value(hi_key);
-            auto in = [&](float v) { return v >= lo && v <= hi; };
-            for (int i0 = 0; i0 < R.n4; i0 += NT) {
-                const float4 v = i0 + tid < R.n4 ? R.four<RESIDENT>(i0 + tid) : make_float4(NAN, NAN, NAN, NAN);
-                const int mine = (int)in(v.x) + in(v.y) + in(v.z) + in(v.w);
-                if (!__any_sync(0xffffffffu, mine)) continue;
-                int at = mine;               // a place for each lane's in the warp's run
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int x = __shfl_up_sync(0xffffffffu, at, o);
-                    if (lane >= o) at += x;
-                }
-                uint32_t base = 0;
-                if (lane == 31) base = atomicAdd(&sm.n_cand, (uint32_t)at);
-                uint32_t to = __shfl_sync(0xffffffffu, base, 31) + at - mine;
-                auto put = [&](float x) {
-                    if (in(x)) {
-                        if (to < CANDS) sm.cand[to] = order_key(x);
-                        to++;
-                    }
-                };
-                put(v.x);
-                put(v.y);
-                put(v.z);
-                put(v.w);
-            }
+            list_bin<NT, RESIDENT>(sm, key_value(lo_key), key_value(hi_key));
             cluster.sync();
             // by a warp, for all
             if (warp == 0) {
@@ -609,6 +649,8 @@ __global__ void __launch_bounds__(NT, FS_OCC(NT)) k_sample_filtered(const float 
     R.a = T > 0.f ? fmax(1.4426950408889634 / (double)T, 1e-300) : 1.0;   // an infinite temperature leaves -infinity behind
     R.half = half;
     R.table = sm.table;
+    if (tid == 0) sm.row = R;
+    __syncthreads();
     // tau, and how many of the elements equal to it stay
     uint32_t tau = 0;
     long long ties = 0, above, goal, own = -1;
@@ -643,26 +685,9 @@ __global__ void __launch_bounds__(NT, FS_OCC(NT)) k_sample_filtered(const float 
     // ---- the draw
     const float ft = tau ? key_value(tau) : -INFINITY;   // (no filter: -infinity's weight is 0, kept or not)
     const long long wtau = tau ? R.units(ft) : 0;
-    auto part = [&](int b, int e) {          // a warp's fours b .. e - 1: their weight above tau, and ties
-        long long mass = 0;
-        int tie = 0;
-        for (int i = b + lane; i < e; i += 32) {
-            const float4 v = R.four<RESIDENT>(i);
-            tie += (int)(v.x == ft) + (int)(v.y == ft) + (int)(v.z == ft) + (int)(v.w == ft);
-            if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) > ft)) continue;
-            const long long w0 = R.units(v.x), w1 = R.units(v.y), w2 = R.units(v.z), w3 = R.units(v.w);
-            mass += (v.x > ft ? w0 : 0) + (v.y > ft ? w1 : 0) + (v.z > ft ? w2 : 0) + (v.w > ft ? w3 : 0);
-        }
-        mass = warp_sum(mass);
-        tie = __reduce_add_sync(0xffffffffu, tie);
-        if (lane == 0) {
-            sm.wsum[warp] = mass;
-            sm.wtie[warp] = tie;
-        }
-    };
     int step = (R.n4 + NW - 1) / NW;
     const bool known = own >= 0;             // the same in every CTA of the cluster
-    if (!none && !known) part(min(R.n4, warp * step), min(R.n4, (warp + 1) * step));
+    if (!none && !known) part<RESIDENT>(sm, min(R.n4, warp * step), min(R.n4, (warp + 1) * step), ft);
     __syncthreads();
     if (tid == 0) {
         long long mass = known ? own : 0;
@@ -703,7 +728,7 @@ __global__ void __launch_bounds__(NT, FS_OCC(NT)) k_sample_filtered(const float 
     // from the slice to a warp's part of it, to a warp's part of that, to the element
     int b = 0, len = R.n4;
     for (int level = 0; level < 2; level++) {
-        if (level || known) part(min(b + len, b + warp * step), min(b + len, b + (warp + 1) * step));
+        if (level || known) part<RESIDENT>(sm, min(b + len, b + warp * step), min(b + len, b + (warp + 1) * step), ft);
         __syncthreads();
         if (warp == 0) {
             const long long mass = lane < NW ? sm.wsum[lane] : 0, tie = lane < NW ? sm.wtie[lane] : 0;
