@@ -28,8 +28,7 @@
 #include <cmath>
 
 #include "hd_internal.cuh"
-#include "hd_kv4.cuh"
-#include "hd_kv4_args.cuh"
+#include "hd_kv4_math.cuh"
 #include "hd_mma.cuh"
 
 namespace {
@@ -80,26 +79,6 @@ __device__ __forceinline__ int d_slot(int p) {
 template <int HD>
 __device__ __forceinline__ int d_piece(int slot, int c) { return HD == 128 ? c ^ (slot & 2) : c; }
 
-// (nibble - 8) * d for the pairs of a word: nibbles 0 and 4, 2 and 6 (odd
-// bytes), and 1 and 5, 3 and 7 (the bytes' high halves); exact.
-__device__ __forceinline__ uint32_t hmul2u(uint32_t a, uint32_t b) {
-    __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
-    return *reinterpret_cast<uint32_t *>(&r);
-}
-// `magic` is H_MAGIC from a register that the compiler cannot see through: as
-// a constant, mask and magic are two immediates and take two instructions.
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
-    return r;
-}
-__device__ __forceinline__ uint32_t nib_lo(uint32_t w, uint32_t d2, uint32_t magic) {
-    return hmul2u(hsub2u(and_or(w, 0x000F000Fu, magic), 0x64086408u), d2);                // 1024 + n - 1032
-}
-__device__ __forceinline__ uint32_t nib_hi(uint32_t w, uint32_t d2, uint32_t magic) {
-    return hmul2u(hfma2u(and_or(w, 0x00F000F0u, magic), H_SIXTEENTH, 0xD480D480u), d2);   // (1024 + 16 n) / 16 - 72
-}
-
 // d += a b, m16n8k16, in place.
 __device__ __forceinline__ void mma_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -125,40 +104,10 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[N]) {
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(a));
 }
 
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t *>(&h);
-}
-// (a, b) in two f16 parts.
-__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = pack2(a - f.x, b - f.y);
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// The tiles a request's last position sees: `sink` first ones, then those from
-// `from` on, `units` in all.
-struct Seen {
-    int last, first;   // the query's position, the window's first one
-    int sink, from, units;
-};
-__device__ __forceinline__ Seen seen_tiles(const Kv4Args &A, int len) {
-    Seen s;
-    const int cap = A.max_pages << A.shift;
-    len = len < 0 ? 0 : len > cap ? cap : len;
-    s.last = len - 1;
-    s.first = A.window && len > A.window ? len - A.window : 0;
-    s.from = s.first / KV4_TILE;
-    const int sinks = min(A.sinks, s.first);
-    s.sink = min((sinks + KV4_TILE - 1) / KV4_TILE, s.from);
-    s.units = len == 0 ? 0 : s.sink + s.last / KV4_TILE - s.from + 1;
-    return s;
+// What a request's last position sees.
+__device__ __forceinline__ Seen last_sees(const Kv4Args &A, int len) {
+    const int last = held_length(A, len) - 1;
+    return seen_tiles(A.window, A.sinks, last, last);
 }
 
 // a / b, without the long division where 32 bits hold both.
@@ -263,13 +212,13 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
     const uint32_t v_at = 8 * HD + vslot * ROW + v_in, v4_at = 8 * HD + vslot4 * ROW + v_in;
     const uint32_t vd_at = 17 * HD + 2 * (t * (HD / 32) + g * (HD / 16) / 16);
     const uint32_t q_at = smem_u32(sm.q[0][lane]);
-    const uint32_t magic = H_MAGIC + (uint32_t)(A.shift >> 8);   // the shift is at most 10
+    const uint32_t magic = KV4_MAGIC + (uint32_t)(A.shift >> 8);   // the shift is at most 10
     const int items = A.n_kv * groups, rep = A.n_heads / A.n_kv;
 
     // ---- this CTA's run of units
     const int per_thread = (A.seqs + DNT - 1) / DNT, rb = min(A.seqs, tid * per_thread), re = min(A.seqs, rb + per_thread);
     int64_t mine = 0;
-    for (int r = rb; r < re; r++) mine += cost_of(seen_tiles(A, A.lens[r]));
+    for (int r = rb; r < re; r++) mine += cost_of(last_sees(A, A.lens[r]));
     int64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -291,13 +240,13 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
     const int64_t c_begin = per * blockIdx.x, c_end = min(total, c_begin + per);
     // requests without any position
     for (int r = blockIdx.x; r < A.seqs; r += gridDim.x)
-        if (seen_tiles(A, A.lens[r]).units == 0)
+        if (last_sees(A, A.lens[r]).units == 0)
             for (int i = tid; i < A.n_heads * HD; i += DNT) A.out[(int64_t)r * A.n_heads * HD + i] = 0.f;
     if (c_begin >= c_end) return;
     if (before <= c_begin && c_begin < before + mine * items) {
         int r = rb;
         for (;; r++) {
-            const int64_t u = (int64_t)cost_of(seen_tiles(A, A.lens[r])) * items;
+            const int64_t u = (int64_t)cost_of(last_sees(A, A.lens[r])) * items;
             if (c_begin < before + u) break;
             before += u;
         }
@@ -309,7 +258,7 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
     int64_t off = sm.start_off;
 
     for (int64_t at = c_begin; at < c_end;) {
-        const Seen S = seen_tiles(A, A.lens[req]);
+        const Seen S = last_sees(A, A.lens[req]);
         const int cost = cost_of(S);
         if (off >= (int64_t)cost * items) {
             off -= (int64_t)cost * items;
@@ -347,11 +296,9 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
             }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // 2^(14 - exponent of mx), a normal number as its inverse is
-            int e = (int)(__float_as_uint(mx) >> 23) - 127;
-            e = e < -100 ? -100 : e;
-            const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-            if (t == 0) sm.kappa[g] = A.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+            float up, kappa;
+            q_scales(mx, A.scale, up, kappa);
+            if (t == 0) sm.kappa[g] = kappa;
 #pragma unroll
             for (int w = 0; w < WPT; w++)
 #pragma unroll
@@ -371,7 +318,7 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
         auto look = [&](int batch) {
             const int u = first_u + DPT * DW * (16 * batch + (lane >> 1)) + (lane & 1);
             if (u >= u1) return -1;
-            const int tile = u < S.sink ? u : S.from + u - S.sink;
+            const int tile = S.tile(u);
             const int64_t page = table[tile >> (A.shift - 4)];
             if (page < 0 || page >= A.pages) return -1;
             return (int)(((page * A.n_kv + kvh) << (A.shift - 4)) + (tile & ((1 << (A.shift - 4)) - 1)));
@@ -429,9 +376,8 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
             // their slots hold counts for nothing (their scores are hidden below)
             uint32_t hidden = 0;        // bit 16 j + p: position p of tile j is not seen
             if (!whole) {
-                const int j = lane >> 4, p = lane & 15, uu = u + j;
-                const int at = (uu < S.sink ? uu : S.from + uu - S.sink) * KV4_TILE + p;
-                const bool sees = (ok >> j & 1) && at <= S.last && (at >= S.first || at < A.sinks);
+                const int j = lane >> 4, p = lane & 15;
+                const bool sees = (ok >> j & 1) && S.any(S.tile(u + j) * KV4_TILE + p, A.sinks);
                 if (!sees) {
                     uint8_t *d = sm.ring[warp][cur][j] + 16 * HD + p * (HD / 16);
 #pragma unroll

@@ -1,0 +1,563 @@
+// hd_kv4_prefill.cu -- causal attention of prompt chunks over the paged 4-bit
+// cache on the tcgen05 tensor cores.
+//
+// A CTA takes 128 query rows -- the heads of one kv head for as many
+// consecutive tokens of a request as fit -- and walks the positions that any
+// of them sees, 128 at a time.  Operands and accuracy are those of the decode
+// kernel: cache values are exact in f16, q and the softmax weights enter in
+// two f16 parts, so each product is two MMAs into the same f32 accumulator.
+//   S = Qhi K^T + Qlo K^T      A = Q in shared memory, B = K [128][HD]
+//   O += Phi V + Plo V         A = P in tensor memory, B = V^T [HD][128]
+//
+// Roles (13 warps, one CTA per SM):
+//   warps 0-3, 4-7  two softmax streams; stream s takes the position tiles
+//            j = s, s + 2, ...  Each has its own S, P, O, maximum and sum, so
+//            while one stream's products run the other computes weights, and
+//            the two join at the end.  A thread owns a row.  P overwrites S in
+//            place: 32 scores become 16 + 16 columns of high and low parts.
+//   warps 8-11      read cache tiles and write K and V^T as f16 operands in
+//            SWIZZLE_128B; a tile's raw words are in registers before its
+//            stage is free.  K's dimensions keep the order in which nibbles
+//            unpack and Q is stored to match; V is paired by byte permutes, so
+//            neither is transposed through memory.
+//   warp 12         issues the MMAs.
+//
+// The maximum is followed lazily: weights are 2^(s - ref + 7) with ref at most
+// 8 below the row's maximum, so they stay below 2^15 in f16, and O is rescaled
+// in tensor memory only when ref moves.  The smallest weight that still counts
+// is 2^-32 of the largest.
+//
+// A value that is not finite (a cache row quantized from a NaN) must reach the
+// rows that see its position and no other, but 0 * NaN is NaN: such values
+// enter V as 0 and are kept in a bit mask per position, which the rows that
+// see it take over for their output dimensions.
+#include "hd_internal.cuh"
+#include "hd_kv4_math.cuh"
+#include "hd_tc.cuh"
+
+namespace {
+
+constexpr int PM = 128, PN = 128;               // rows, positions per tile
+constexpr int P_SOFT = 256, P_DEQ = 128;        // threads of the softmax streams and of the unpacking warps
+constexpr int P_THREADS = P_SOFT + P_DEQ + 32;
+constexpr int PG = PN / KV4_TILE;               // cache tiles per position tile
+constexpr int ABSENT = 0x40000000;              // position of a cache tile that is not there
+
+template <int HD>
+struct PLayout {
+    static constexpr int ATOMS = HD > 64 ? HD / 64 : 1;      // 128-byte columns of a row of K and Q
+    static constexpr int Q = PM * 128 * ATOMS, K = PN * 128 * ATOMS, V = HD * 256;
+    static constexpr int OPERANDS = 2 * Q + 2 * (K + V);
+    // at least half an SM's shared memory: a second CTA would wait for tensor memory
+    static constexpr size_t BYTES = (OPERANDS > 120 * 1024 ? OPERANDS : 120 * 1024) + 1024;
+};
+
+struct PShared {
+    unsigned long long kv_full[2], s_full[2], p_full[2], pv_done[2], fin;
+    uint32_t tmem;
+    int pos[2][PG];               // first position of each cache tile of a stage
+    uint32_t nan_of[2][PN];       // groups of V that are not finite, per position
+    int nan_any[2];
+    float m[2][PM], l[2][PM], mx[2][PM];
+    uint32_t nan_row[2][PM];
+    int64_t part[P_THREADS / 32];
+    int req, tile, found;
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(a));
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; i++) asm volatile("" : "+r"(r[i])::"memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool not_finite(uint32_t d) { return (d & 0x7fffu) >= 0x7c00u; }
+
+template <int HD>
+__global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq, int *flag) {
+    using L = PLayout<HD>;
+    constexpr int KS = HD / 16;                            // k-steps of the first product
+    constexpr uint32_t S_COL = 0, O_COL = 2 * PN;          // tensor memory: S and P of both streams, then O of both
+    extern __shared__ uint8_t raw[];
+    __shared__ PShared sm;
+    uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t q_hi = smem_u32(base), q_lo = q_hi + L::Q, kv0 = q_lo + L::Q;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- which rows: query tiles of all requests in one line, the last first (they see most)
+    const int kvh = blockIdx.x % A.n_kv, index = blockIdx.x / A.n_kv, rep = A.n_heads / A.n_kv;
+    {
+        auto tiles_of = [&](int r) { return (max(0, A.row0[r + 1] - A.row0[r]) + tq - 1) / tq; };
+        const int per = (A.seqs + P_THREADS - 1) / P_THREADS, b = min(A.seqs, tid * per), e = min(A.seqs, b + per);
+        int64_t mine = 0;
+        for (int r = b; r < e; r++) mine += tiles_of(r);
+        int64_t inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += x;
+        }
+        if (lane == 31) sm.part[warp] = inc;
+        if (tid == 0) sm.found = 0;
+        __syncthreads();
+        int64_t at = inc - mine, total = 0;
+        for (int w = 0; w < P_THREADS / 32; w++) {
+            if (w < warp) at += sm.part[w];
+            total += sm.part[w];
+        }
+        const int64_t want = total - 1 - index;
+        if (want >= at && want < at + mine) {
+            int r = b;
+            for (;; r++) {
+                const int t = tiles_of(r);
+                if (want < at + t) break;
+                at += t;
+            }
+            sm.req = r;
+            sm.tile = (int)(want - at);
+            sm.found = 1;
+        }
+        __syncthreads();
+        if (!sm.found) return;
+    }
+    const int req = sm.req, r_begin = A.row0[req], n_new = A.row0[req + 1] - r_begin, t0 = sm.tile * tq;
+    const int tokens = min(tq, n_new - t0), rows = tokens * rep;
+    const int i0 = held_length(A, A.lens[req]) - n_new + t0;      // the first token's position (below 0: it sees nothing)
+    const Seen S = seen_tiles(A.window, A.sinks, i0, i0 + tokens - 1);
+    const int nj = (S.units + PG - 1) / PG;
+    const int32_t *table = A.tables + (int64_t)req * A.max_pages;
+    // (rows beyond the buffers, which row0 may name, are neither read nor written)
+    auto row_ok = [&](int r) { return r < rows && r_begin >= 0 && (int64_t)r_begin + t0 + r / rep < A.rows; };
+
+    if (tid == 0) {
+        for (int s = 0; s < 2; s++) {
+            mbar_init(smem_u32(&sm.kv_full[s]), P_DEQ);
+            mbar_init(smem_u32(&sm.s_full[s]), 1);
+            mbar_init(smem_u32(&sm.p_full[s]), P_SOFT / 2);
+            mbar_init(smem_u32(&sm.pv_done[s]), 1);
+            sm.nan_any[s] = 0;
+        }
+        mbar_init(smem_u32(&sm.fin), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (tid < 2 * PN) sm.nan_of[tid / PN][tid % PN] = 0;
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // ---- Q: rows of the first warps' threads, half of the 16-byte chunks each
+    float kappa = 0.f;
+    const int r = tid & (PM - 1), half = tid >> 7;
+    if (tid < P_SOFT) {
+        constexpr int CH = HD / 16;                        // chunks of 8 dimensions per thread
+        float4 x[CH][2];
+        const float *q = A.q + ((int64_t)r_begin + t0 + r / rep) * A.q_ld + (int64_t)(kvh * rep + r % rep) * HD;
+        const bool ok = row_ok(r);
+        float mx = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int ch = half * CH + c, d = ch / 4 * 32 + 4 * (ch % 4);
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                x[c][y] = ok ? *(const float4 *)(q + d + 16 * y) : make_float4(0.f, 0.f, 0.f, 0.f);
+                mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[c][y].x), fabsf(x[c][y].y)), fmaxf(fabsf(x[c][y].z), fabsf(x[c][y].w))));
+            }
+        }
+        sm.mx[half][r] = mx;
+        bar_sync(1, P_SOFT);
+        float up;
+        q_scales(fmaxf(sm.mx[0][r], sm.mx[1][r]), A.scale, up, kappa);
+        kappa = fmaxf(kappa, 1e-37f);                      // -infinity * kappa stays -infinity
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int ch = half * CH + c;
+            uint4 hi, lo;
+            split2(x[c][0].x * up, x[c][0].z * up, hi.x, lo.x);
+            split2(x[c][0].y * up, x[c][0].w * up, hi.y, lo.y);
+            split2(x[c][1].x * up, x[c][1].z * up, hi.z, lo.z);
+            split2(x[c][1].y * up, x[c][1].w * up, hi.w, lo.w);
+            const int at = (ch >> 3) * (PM * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+            *(uint4 *)(base + at) = hi;
+            *(uint4 *)(base + L::Q + at) = lo;
+        }
+        fence_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+
+    if (warp < 8) {
+        // ================= softmax stream s
+        const int s = half;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t t_s = tmem + lanes + S_COL + s * PN, t_o = tmem + lanes + O_COL + s * HD;
+        const int i_row = i0 + r / rep, f_row = A.window && i_row >= A.window ? i_row - A.window + 1 : 0;
+        const int n = (nj - s + 1) / 2;                    // this stream's tiles
+        float m = -INFINITY, l = 0.f;
+        uint32_t nan_mine = 0;
+        bool alive = true;
+        for (int k = 0; k < n && alive; k++) {
+            alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.kv_full[s]), k & 1, flag) &&
+                                                mbar_wait(smem_u32(&sm.s_full[s]), k & 1, flag));
+            if (!alive) break;
+            tc_fence_after();
+            // scores of 32 columns, -infinity where the row does not see the position
+            auto load = [&](int c, float (&v)[32]) {
+                uint32_t (&u)[32] = reinterpret_cast<uint32_t (&)[32]>(v);
+                tmem_ld32(t_s + 32 * c, u);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int p0 = sm.pos[s][2 * c + h];
+                    const bool all = p0 + KV4_TILE - 1 <= i_row && (p0 >= f_row || p0 + KV4_TILE <= A.sinks);
+                    if (__all_sync(0xffffffffu, all)) continue;
+#pragma unroll
+                    for (int i = 0; i < KV4_TILE; i++) {
+                        const int p = p0 + i;
+                        if (!(p <= i_row && (p >= f_row || p < A.sinks))) v[16 * h + i] = -INFINITY;
+                    }
+                }
+            };
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                float v[32];
+                load(c, v);
+                float a = v[0], b = v[1];
+#pragma unroll
+                for (int i = 2; i < 32; i += 2) {
+                    a = fmaxf(a, v[i]);
+                    b = fmaxf(b, v[i + 1]);
+                }
+                mx = fmaxf(mx, fmaxf(a, b));
+            }
+            mx *= kappa;
+            const bool moves = mx > m + 8.f || (m == -INFINITY && mx > -INFINITY);
+            if (__any_sync(0xffffffffu, moves && m > -INFINITY)) {
+                // O in tensor memory follows; the stream's last product is done before it changes
+                alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), (k - 1) & 1, flag));
+                if (!alive) break;
+                tc_fence_after();
+                const float a = moves && m > -INFINITY ? exp2_approx(m - mx) : 1.f;
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; c++) {
+                    uint32_t o[32];
+                    tmem_ld32(t_o + 32 * c, o);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
+                    tmem_st32(t_o + 32 * c, o);
+                }
+                l *= a;
+            }
+            if (moves) m = mx;
+            const float ref = m == -INFINITY ? 0.f : m - 7.f;
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                float v[32];
+                load(c, v);
+                uint32_t p[32];
+                float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float a = exp2_approx(fmaf(v[2 * i], kappa, -ref)), b = exp2_approx(fmaf(v[2 * i + 1], kappa, -ref));
+                    l0 += a;
+                    l1 += b;
+                    split2(a, b, p[i], p[16 + i]);
+                }
+                l += l0 + l1;
+                tmem_st32(t_s + 32 * c, p);
+            }
+            if (sm.nan_any[s]) {                           // the same for the whole stream
+                for (int i = 0; i < PN; i++) {
+                    const int p = sm.pos[s][i / KV4_TILE] + i % KV4_TILE;
+                    if (p <= i_row && (p >= f_row || p < A.sinks)) nan_mine |= sm.nan_of[s][i];
+                }
+                bar_sync(2 + s, P_SOFT / 2);
+                sm.nan_of[s][r] = 0;
+                if (r == 0) sm.nan_any[s] = 0;
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&sm.p_full[s]));
+        }
+        // ---- the streams join; each writes half of the dimensions
+        sm.m[s][r] = m;
+        sm.l[s][r] = l;
+        sm.nan_row[s][r] = nan_mine;
+        const int n0 = (nj + 1) / 2, n1 = nj / 2;
+        if (alive && n0 > 0) alive = mbar_wait(smem_u32(&sm.pv_done[0]), (n0 - 1) & 1, flag);
+        if (alive && n1 > 0) alive = mbar_wait(smem_u32(&sm.pv_done[1]), (n1 - 1) & 1, flag);
+        tc_fence_after();
+        bar_sync(1, P_SOFT);
+        const float m0 = sm.m[0][r], m1 = sm.m[1][r], M = fmaxf(m0, m1), top = M == -INFINITY ? 0.f : M;
+        const float a0 = exp2_approx(m0 - top), a1 = exp2_approx(m1 - top);
+        const float sum = fmaf(sm.l[0][r], a0, sm.l[1][r] * a1), inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float f0 = a0 * inv, f1 = a1 * inv;
+        const uint32_t nans = sm.nan_row[0][r] | sm.nan_row[1][r];
+        float *out = A.out + (((int64_t)r_begin + t0 + r / rep) * A.n_heads + kvh * rep + r % rep) * HD;
+        const bool ok = row_ok(r);
+        constexpr int W = HD / 2 > 32 ? 32 : 16;           // dimensions at a time
+#pragma unroll 1
+        for (int d0 = s * (HD / 2); d0 < (s + 1) * (HD / 2); d0 += W) {
+            float v[W];
+#pragma unroll
+            for (int i = 0; i < W; i++) v[i] = 0.f;
+            // (all lanes take part in the loads)
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                if ((y ? n1 : n0) == 0 || !alive) continue;
+                const uint32_t at = tmem + lanes + O_COL + y * HD + d0;
+#pragma unroll
+                for (int z = 0; z < W; z += 16) {
+                    uint32_t o[16];
+                    tmem_ld16_async(at + z, o);
+                    tmem_wait_ld();
+                    tmem_regs_ready(o);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) v[z + i] = fmaf(__uint_as_float(o[i]), y ? f1 : f0, v[z + i]);
+                }
+            }
+            if (!ok || !alive) continue;
+            const bool bad = nans >> (d0 / 32) & 1;
+#pragma unroll
+            for (int i = 0; i < W; i += 4)
+                *(float4 *)(out + d0 + i) = i_row < 0 || sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                            : bad ? make_float4(NAN, NAN, NAN, NAN)
+                                                  : make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
+    } else if (warp < 12) {
+        // ================= cache tiles to operands
+        const int w4 = warp - 8;
+        const uint32_t magic = KV4_MAGIC + (uint32_t)(A.shift >> 8);   // the shift is at most 10
+        constexpr int PIECES = HD / 32, KROWS = 32 / PIECES, KI = PN / (4 * KROWS);
+        const int k_piece = lane / KROWS, k_row = w4 * KROWS + lane % KROWS;
+        // V: 8 positions x VW words of one 16-byte piece
+        constexpr int VW = HD == 128 ? 2 : 1;
+        const int vr = w4 * 4 + (lane >> 3), v_atom = vr & 1, v_chunk = (lane & 7) | (v_atom << 3);
+        const int v_piece = HD == 32 ? 0 : (vr >> 1) & (PIECES - 1);
+        const int v_word = HD == 128 ? 2 * (vr >> 3) : HD == 64 ? vr >> 2 : (vr >> 1) & 3;
+        const bool v_on = HD != 32 || vr < 8;
+        const int page_tiles = 1 << (A.shift - 4);
+        // lane i < 8: where cache tile i of position tile j lies, or -1; and its first position
+        auto look = [&](int j, int &pos) {
+            const int u = PG * j + (lane & 7);
+            pos = ABSENT;
+            if (u >= S.units) return -1;
+            const int tile = S.tile(u);
+            const int64_t page = table[tile >> (A.shift - 4)];
+            if (page < 0 || page >= A.pages) return -1;
+            pos = tile * KV4_TILE;
+            return (int)((page * A.n_kv + kvh) * page_tiles + (tile & (page_tiles - 1)));
+        };
+        uint4 kw[KI];
+        uint32_t kd[KI], vw[8][VW], vd[8];
+        int pos = ABSENT;
+        auto fetch = [&](int at) {
+#pragma unroll
+            for (int i = 0; i < KI; i++) {
+                const int row = i * 4 * KROWS + k_row, tile = __shfl_sync(0xffffffffu, at, row / KV4_TILE);
+                const int p = __shfl_sync(0xffffffffu, pos, row / KV4_TILE) + row % KV4_TILE;
+                kw[i] = make_uint4(0, 0, 0, 0);
+                kd[i] = 0;
+                if (tile >= 0 && S.any(p, A.sinks)) {
+                    const uint8_t *src = A.cache + (uint64_t)(uint32_t)tile * kv4_tile_bytes(HD);
+                    kw[i] = __ldg((const uint4 *)(src + (row % KV4_TILE) * (HD / 2) + 16 * k_piece));
+                    kd[i] = __ldg((const uint16_t *)(src + 16 * HD) + (row % KV4_TILE) * PIECES + k_piece);
+                }
+            }
+            const int g = v_chunk >> 1, tile = __shfl_sync(0xffffffffu, at, g), p0 = __shfl_sync(0xffffffffu, pos, g) + 8 * (v_chunk & 1);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                vd[i] = 0;
+#pragma unroll
+                for (int w = 0; w < VW; w++) vw[i][w] = 0;
+                if (v_on && tile >= 0 && S.any(p0 + i, A.sinks)) {
+                    const int row = 8 * (v_chunk & 1) + i;
+                    const uint8_t *src = A.cache + (uint64_t)(uint32_t)tile * kv4_tile_bytes(HD);
+                    const uint32_t *q = (const uint32_t *)(src + 8 * HD + row * (HD / 2) + 16 * v_piece) + v_word;
+                    if constexpr (VW == 2) {
+                        const uint2 x = __ldg((const uint2 *)q);
+                        vw[i][0] = x.x;
+                        vw[i][1] = x.y;
+                    } else {
+                        vw[i][0] = __ldg(q);
+                    }
+                    vd[i] = __ldg((const uint16_t *)(src + 17 * HD) + row * PIECES + v_piece);
+                }
+            }
+        };
+        int at = nj > 0 ? look(0, pos) : -1, pos_next = ABSENT;
+        int at_next = nj > 1 ? look(1, pos_next) : -1;
+        if (nj > 0) fetch(at);
+        for (int j = 0; j < nj; j++) {
+            const int s = j & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), ((j >> 1) & 1) ^ 1, flag))) break;
+            uint8_t *K = base + 2 * L::Q + s * (L::K + L::V), *V = K + L::K;
+            if (w4 == 0 && lane < PG) sm.pos[s][lane] = pos;
+#pragma unroll
+            for (int i = 0; i < KI; i++) {
+                const int row = i * 4 * KROWS + k_row;
+                const uint32_t d = __byte_perm(kd[i], kd[i], 0x1010);
+                const uint32_t w[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const uint32_t w8 = w[c] >> 8;
+                    const int ch = 4 * k_piece + c;
+                    *(uint4 *)(K + (ch >> 3) * (PN * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
+                        make_uint4(nib_lo(w[c], d, magic), nib_lo(w8, d, magic), nib_hi(w[c], d, magic), nib_hi(w8, d, magic));
+                }
+            }
+            if (v_on) {
+                uint32_t dd[4];
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < 8; i++) odd = odd || not_finite(vd[i]);
+                if (odd) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (not_finite(vd[i])) {
+                            vd[i] = 0;
+                            atomicOr(&sm.nan_of[s][8 * v_chunk + i], 1u << v_piece);
+                            sm.nan_any[s] = 1;
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) dd[i] = __byte_perm(vd[2 * i], vd[2 * i + 1], 0x5410);
+                const uint32_t chunk = lane & 7;
+#pragma unroll
+                for (int w = 0; w < VW; w++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {          // bytes 2 h, 2 h + 1 of the word
+                        uint32_t x[4], y[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            x[i] = __byte_perm(vw[2 * i][w], vw[2 * i + 1][w], h ? 0x7632 : 0x5410);
+                            y[i] = x[i] >> 8;
+                        }
+                        const uint32_t dim = 32 * v_piece + 4 * (v_word + w) + 2 * h;
+                        auto put = [&](uint32_t row, uint4 v) {
+                            *(uint4 *)(V + v_atom * (HD * 128) + row * 128 + ((chunk ^ (row & 7)) << 4)) = v;
+                        };
+                        put(dim, make_uint4(nib_lo(x[0], dd[0], magic), nib_lo(x[1], dd[1], magic), nib_lo(x[2], dd[2], magic), nib_lo(x[3], dd[3], magic)));
+                        put(dim + 1, make_uint4(nib_lo(y[0], dd[0], magic), nib_lo(y[1], dd[1], magic), nib_lo(y[2], dd[2], magic), nib_lo(y[3], dd[3], magic)));
+                        put(dim + 16, make_uint4(nib_hi(x[0], dd[0], magic), nib_hi(x[1], dd[1], magic), nib_hi(x[2], dd[2], magic), nib_hi(x[3], dd[3], magic)));
+                        put(dim + 17, make_uint4(nib_hi(y[0], dd[0], magic), nib_hi(y[1], dd[1], magic), nib_hi(y[2], dd[2], magic), nib_hi(y[3], dd[3], magic)));
+                    }
+            }
+            fence_async_smem();
+            mbar_arrive(smem_u32(&sm.kv_full[s]));
+            if (j + 1 < nj) {
+                at = at_next;
+                pos = pos_next;
+                fetch(at);
+                at_next = j + 2 < nj ? look(j + 2, pos_next) : -1;
+            }
+        }
+    } else if (lane == 0) {
+        // ================= MMAs
+        constexpr uint32_t id_s = idesc_f16(PN), id_o = idesc_f16(HD);
+        auto values = [&](int j) {                         // O += P V of tile j
+            const int s = j & 1, k = j >> 1;
+            if (!mbar_wait(smem_u32(&sm.p_full[s]), k & 1, flag)) return false;
+            tc_fence_after();
+            const uint32_t v0 = kv0 + s * (L::K + L::V) + L::K, p0 = tmem + S_COL + s * PN, d = tmem + O_COL + s * HD;
+#pragma unroll
+            for (int ks = 0; ks < PN / 16; ks++) {
+                const uint64_t bd = sw128_desc(v0 + (ks >> 2) * (HD * 128) + (ks & 3) * 32);
+                const uint32_t a = p0 + 32 * (ks >> 1) + 8 * (ks & 1);
+                mma_ts(d, a, bd, id_o, k > 0 || ks > 0);
+                mma_ts(d, a + 16, bd, id_o, 1);
+            }
+            commit(smem_u32(&sm.pv_done[s]));
+            return true;
+        };
+        bool alive = true;
+        for (int j = 0; j < nj && alive; j++) {
+            const int s = j & 1;
+            alive = mbar_wait(smem_u32(&sm.kv_full[s]), (j >> 1) & 1, flag);
+            if (!alive) break;
+            tc_fence_after();
+            const uint32_t k0 = kv0 + s * (L::K + L::V), d = tmem + S_COL + s * PN;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const uint32_t off = (ks >> 2) * (PM * 128) + (ks & 3) * 32;
+                const uint64_t bd = sw128_desc(k0 + off);
+                mma_ss(d, sw128_desc(q_hi + off), bd, id_s, ks > 0);
+                mma_ss(d, sw128_desc(q_lo + off), bd, id_s, 1);
+            }
+            commit(smem_u32(&sm.s_full[s]));
+            if (j > 0) alive = values(j - 1);
+        }
+        if (alive && nj > 0) alive = values(nj - 1);
+        // what was issued ends before tensor memory is freed, also after a wait that ran out
+        commit(smem_u32(&sm.fin));
+        mbar_wait_quiet(smem_u32(&sm.fin), 0);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+template <int HD>
+cudaError_t launch(hd_ctx *ctx, const Kv4Args &A) {
+    constexpr size_t smem = PLayout<HD>::BYTES;
+    cudaError_t e = cudaFuncSetAttribute(k_kv4_prefill<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    const int rep = A.n_heads / A.n_kv, tq = PM / rep;
+    // a request's last tile may be short: at most one more tile each, and no more than rows
+    int64_t tiles = A.rows / tq + A.seqs;
+    tiles = tiles < A.rows ? tiles : A.rows;
+    return hd_launch(ctx, k_kv4_prefill<HD>, dim3((unsigned)(tiles * A.n_kv)), dim3(P_THREADS), smem, A, tq, ctx->flag);
+}
+
+}  // namespace
+
+extern "C" int hd_kv4_attention_prefill(hd_ctx *ctx, const float *q, int64_t q_ld, const uint8_t *cache, int64_t pages,
+                                        int page_size, const int32_t *tables, int max_pages, const int32_t *lens,
+                                        const int32_t *row0, int seqs, int64_t rows, int n_heads, int n_kv, int head_dim,
+                                        int window, int sinks, float scale, float *out) {
+    Kv4Args A{q, q_ld, cache, pages, 0, tables, max_pages, lens, row0, seqs, rows, n_heads, n_kv, window, sinks, scale, out};
+    if (seqs > 0 && !row0) return hd_fail(ctx, HD_E_ARG, "hd_kv4_attention_prefill: null argument");
+    int rc = hd_kv4_attention_check(ctx, "hd_kv4_attention_prefill", A, page_size, head_dim);
+    if (rc || seqs == 0 || rows == 0) return rc;
+    HD_REQUIRE(ctx, (rows + seqs) * n_kv < ((int64_t)1 << 31), HD_E_SHAPE, "hd_kv4_attention_prefill: %lld rows of %d kv heads",
+               (long long)rows, n_kv);
+    HdDevice on(ctx);
+    cudaError_t e = head_dim == 128 ? launch<128>(ctx, A) : head_dim == 64 ? launch<64>(ctx, A) : launch<32>(ctx, A);
+    if (e != cudaSuccess) return hd_fail(ctx, HD_E_CUDA, "hd_kv4_attention_prefill: %s", cudaGetErrorString(e));
+    return HD_OK;
+}

@@ -69,7 +69,7 @@ def seen(i, n, window, sinks):
     return ok
 
 
-def attention(q, k, v, ok, scale):
+def attention(q, k, v, ok, scale, floor=2.0 ** -40):
     """q [heads, hd], k and v [n, n_kv, hd] float64 -> (out [heads, hd], bound on a float32 kernel's error).
 
     The bound: a score is a dot product of hd float32 products, so it is off by
@@ -79,10 +79,12 @@ def attention(q, k, v, ok, scale):
     of n terms in float32 by n / 4 + 64 roundings (partial sums of at least
     four parallel accumulators, then their merge) of 2^-24 of sum p |v|, for
     the numerator and for the denominator.  A weight enters its product in two
-    f16 parts after a scaling of the largest to 2^15; f16 has no bit below
+    f16 parts after a scaling of the largest to 2^15 (decode) or to between 2^7
+    and 2^15 (prefill, which follows the maximum lazily); f16 has no bit below
     2^-24, so besides its relative error each weight is off by up to half of
-    that, 2^-25 / 2^15 = 2^-40 of the largest weight, times its |v|: what a
-    dimension shows whose heavy positions all hold a zero."""
+    that, `floor` = 2^-25 / 2^15 = 2^-40 (or 2^-25 / 2^7 = 2^-32) of the largest
+    weight, times its |v|: what a dimension shows whose heavy positions all
+    hold a zero."""
     heads, hd = q.shape
     rep = heads // k.shape[1]
     out, tol = np.zeros((heads, hd)), np.zeros((heads, hd))
@@ -96,7 +98,7 @@ def attention(q, k, v, ok, scale):
         p /= p.sum()
         out[h] = p @ vv
         tol[h] = (p @ np.abs(vv)) * (2 * ds + 2.0 ** -21 + 2 * (len(s) / 4 + 64) * 2.0 ** -24) \
-            + 2.0 ** -40 * p.max() * np.abs(vv).sum(0)
+            + floor * p.max() * np.abs(vv).sum(0)
     return out, tol
 
 

@@ -51,12 +51,12 @@ class Case:
         take = lambda q, d: R.values(q[ids], d[ids]).transpose(0, 2, 1, 3).reshape(-1, self.n_kv, self.hd)[:n]  # noqa: E731
         return take(self.kq, self.kd), take(self.vq, self.vd)
 
-    def expect(self, r, q, i, window, sinks, scale=0.0):
+    def expect(self, r, q, i, window, sinks, scale=0.0, floor=2.0 ** -40):
         n = i + 1
         ok = R.seen(i, n, window, sinks)
         named = np.repeat((self.tables[r] >= 0) & (self.tables[r] < self.pages), self.page)[:n]
         k, v = self.kv(r, n)
-        return R.attention(q.astype(np.float64), k, v, ok & named, scale or self.hd ** -0.5)
+        return R.attention(q.astype(np.float64), k, v, ok & named, scale or self.hd ** -0.5, floor)
 
 
 def _close(got, ref, tol):
@@ -240,7 +240,7 @@ def _check_prefill(ctx, torch, c, heads, new, window=0, sinks=0, pad=0):
             if i < 0:
                 assert not got[row0[r] + t].any()
             else:
-                _close(got[row0[r] + t], *c.expect(r, q[row0[r] + t], i, window, sinks))
+                _close(got[row0[r] + t], *c.expect(r, q[row0[r] + t], i, window, sinks, floor=2.0 ** -32))
 
 
 @pytest.mark.parametrize("hd", [32, 64, 128])
@@ -283,7 +283,7 @@ def test_prefill_long(ctx):
     for row in [0, 1, 17, 18, 100, 299, 598, 599, 600, 731, 932]:
         r = int(row >= 600)
         i = c.lens[r] - (600, 333)[r] + row - row0[r]
-        _close(got[row], *c.expect(r, q[row], i, 0, 0))
+        _close(got[row], *c.expect(r, q[row], i, 0, 0, floor=2.0 ** -32))
     again = _prefill(ctx, torch, c, 7, [600, 333], q=q)[2]
     assert torch.equal(again, out)
 
@@ -294,5 +294,70 @@ def test_prefill_of_single_tokens_equals_decode(ctx):
     _, q, a = _prefill(ctx, torch, c, 14, [1, 1, 1, 1])
     b = _decode(ctx, torch, c, 14, q=q)[1]
     for r, n in enumerate(c.lens):
-        _, tol = c.expect(r, q[r], n - 1, 0, 0)
+        _, tol = c.expect(r, q[r], n - 1, 0, 0, floor=2.0 ** -32)
         assert np.all(np.abs(a[r].cpu().numpy() - b[r].cpu().numpy()) <= 2 * tol)
+
+
+def test_prefill_a_nan_reaches_the_rows_that_see_it_and_no_other(ctx):
+    """NaN in a value group and in a key of one position: earlier rows and other heads stay as they are."""
+    import torch
+    c = Case(25, [300], 2, 64, 16)
+    pg = lambda j: c.tables[0, j // 16]  # noqa: E731
+    c.vd[pg(150), 1, 150 % 16, 1] = np.nan        # kv head 1, dimensions 32..63
+    c.kd[pg(200), 0, 200 % 16, 0] = np.nan        # kv head 0: every dimension of the rows that see it
+    c.device(torch)
+    _, q, out = _prefill(ctx, torch, c, 4, [300])
+    got = out.cpu().numpy()
+    assert np.isnan(got[150:, 2:, 32:]).all() and not np.isnan(got[150:, 2:, :32]).any()
+    assert np.isnan(got[200:, :2]).all()
+    assert not np.isnan(got[:150]).any() and not np.isnan(got[150:200, :2]).any()
+    for row in (0, 149, 151, 299):
+        ref, tol = c.expect(0, q[row], row, 0, 0, floor=2.0 ** -32)
+        fine = ~np.isnan(got[row])
+        assert np.all(np.abs(got[row] - ref)[fine] <= tol[fine])
+
+
+def test_prefill_with_a_window_rows_outlive_a_nan(ctx):
+    import torch
+    c = Case(26, [400], 1, 32, 16)
+    c.vd[c.tables[0, 100 // 16], 0, 100 % 16, 0] = np.nan
+    c.device(torch)
+    got = _prefill(ctx, torch, c, 2, [400], window=50, sinks=3)[2].cpu().numpy()
+    assert np.isnan(got[100:150]).all() and not np.isnan(got[:100]).any() and not np.isnan(got[150:]).any()
+
+
+@pytest.mark.parametrize("scale", [0.0, 0.5, 1e-3])
+def test_prefill_large_scores_move_the_maximum(ctx, scale):
+    """Keys that grow along the request: the running maximum moves far and often."""
+    import torch
+    c = Case(27, [700], 1, 64, 16)
+    for j in range(700):
+        c.kd[c.tables[0, j // 16], :, j % 16] *= np.float16(1 + j / 64)
+    c.kd = R._bf16(c.kd.astype(np.float32)).astype(np.float16)
+    c.device(torch)
+    row0, q, out = _prefill(ctx, torch, c, 8, [700])
+    if scale:
+        out = torch.empty_like(out)
+        ctx.kv4_attention_prefill(torch.from_numpy(q).cuda(), c.cache, c.t, c.l, torch.from_numpy(row0).cuda(), out, scale=scale)
+    got = out.cpu().numpy()
+    for row in (0, 1, 63, 64, 127, 128, 255, 300, 511, 640, 699):
+        _close(got[row], *c.expect(0, q[row], row, 0, 0, scale, floor=2.0 ** -32))
+
+
+def test_prefill_many_short_requests_and_strided_q(ctx):
+    import torch
+    rng = np.random.default_rng(28)
+    lens = rng.integers(0, 60, 500)
+    new = np.minimum(lens, rng.integers(0, 4, 500)).tolist()
+    c = Case(28, lens, 2, 32, 16).device(torch)
+    row0 = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    fused = torch.randn(row0[-1] + 9, 6 * 32 + 64, device="cuda")
+    q = fused[:, :6 * 32].unflatten(1, (6, 32))
+    a, b = torch.full((len(q), 6, 32), 7.0, device="cuda"), torch.full((len(q), 6, 32), 7.0, device="cuda")
+    ctx.kv4_attention_prefill(q, c.cache, c.t, c.l, torch.from_numpy(row0).cuda(), a)
+    ctx.kv4_attention_prefill(q.contiguous(), c.cache, c.t, c.l, torch.from_numpy(row0).cuda(), b)
+    assert torch.equal(a, b) and bool((a[row0[-1]:] == 7).all())
+    got, qh = a.cpu().numpy(), q.cpu().numpy()
+    for r in range(0, 500, 7):
+        for t in range(new[r]):
+            _close(got[row0[r] + t], *c.expect(r, qh[row0[r] + t], int(lens[r]) - new[r] + t, 0, 0, floor=2.0 ** -32))

@@ -57,7 +57,7 @@ def test_serving_steps(ctx, page, window, sinks):
             for t in range(new[r]):
                 i = len(model[r][0]) - new[r] + t
                 ref, tol = R.attention(x[at + t, :heads * hd].reshape(heads, hd).astype(np.float64), model[r][0][:i + 1],
-                                       model[r][1][:i + 1], R.seen(i, i + 1, window, sinks), hd ** -0.5)
+                                       model[r][1][:i + 1], R.seen(i, i + 1, window, sinks), hd ** -0.5, 2.0 ** -32)
                 assert np.all(np.abs(got[at + t] - ref) <= tol), (step, r, t)
                 checked += 1
             at += new[r]
