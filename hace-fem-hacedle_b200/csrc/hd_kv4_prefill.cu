@@ -7,25 +7,25 @@
 // kernel: cache values are exact in f16, q and the softmax weights enter in
 // two f16 parts, so each product is two MMAs into the same f32 accumulator.
 //   S = Qhi K^T + Qlo K^T      A = Q in shared memory, B = K [128][HD]
-//   O += Phi V + Plo V         A = P in tensor memory, B = V^T [HD][128]
+//   PV = Phi V + Plo V         A = P in tensor memory, B = V^T [HD][128]
+// O itself is kept in registers and takes up a tile's PV with an addition: an
+// accumulator that grew over the whole context lost low bits at every MMA
+// (7e-6 of the result over 8192 positions, 4e-7 now), and the change of the
+// running maximum is one multiplication on the way.
 //
-// Roles (13 warps, one CTA per SM):
-//   warps 0-3, 4-7  two softmax streams; stream s takes the position tiles
-//            j = s, s + 2, ...  Each has its own S, P, O, maximum and sum, so
-//            while one stream's products run the other computes weights, and
-//            the two join at the end.  A thread owns a row.  P overwrites S in
+// Roles (14 warps, one CTA per SM; S, P and PV have two buffers each in tensor
+// memory, K and V two stages in shared memory, so the four work on different
+// tiles at a time):
+//   warps 0-7       softmax: a thread has a row and half of a tile's columns,
+//            and half of the row's dimensions of O; the two threads of a row
+//            exchange their maxima through shared memory.  P overwrites S in
 //            place: 32 scores become 16 + 16 columns of high and low parts.
-//   warps 8-11      read cache tiles and write K and V^T as f16 operands in
-//            SWIZZLE_128B; a tile's raw words are in registers before its
-//            stage is free.  K's dimensions keep the order in which nibbles
-//            unpack and Q is stored to match; V is paired by byte permutes, so
-//            neither is transposed through memory.
-//   warp 12         issues the MMAs.
-//
-// The maximum is followed lazily: weights are 2^(s - ref + 7) with ref at most
-// 8 below the row's maximum, so they stay below 2^15 in f16, and O is rescaled
-// in tensor memory only when ref moves.  The smallest weight that still counts
-// is 2^-32 of the largest.
+//   warps 8-11      fetch cache tiles by bulk copies and write K and V^T as
+//            f16 operands in SWIZZLE_128B.  K's dimensions keep the order in
+//            which nibbles unpack and Q is stored to match; V is paired by byte
+//            permutes, so neither is transposed through memory.
+//   warp 12, 13     issue the MMAs of S and of PV: one thread for both was the
+//            pace (an MMA costs its issuer 60 to 80 cycles, 32 of them a tile).
 //
 // A value that is not finite (a cache row quantized from a NaN) must reach the
 // rows that see its position and no other, but 0 * NaN is NaN: such values
@@ -38,8 +38,8 @@
 namespace {
 
 constexpr int PM = 128, PN = 128;               // rows, positions per tile
-constexpr int P_SOFT = 256, P_DEQ = 128;        // threads of the softmax streams and of the unpacking warps
-constexpr int P_THREADS = P_SOFT + P_DEQ + 32;
+constexpr int P_SOFT = 256, P_DEQ = 128;        // threads of the softmax and of the unpacking warps
+constexpr int P_THREADS = P_SOFT + P_DEQ + 64;
 constexpr int PG = PN / KV4_TILE;               // cache tiles per position tile
 constexpr int ABSENT = 0x40000000;              // position of a cache tile that is not there
 
@@ -47,19 +47,21 @@ template <int HD>
 struct PLayout {
     static constexpr int ATOMS = HD > 64 ? HD / 64 : 1;      // 128-byte columns of a row of K and Q
     static constexpr int Q = PM * 128 * ATOMS, K = PN * 128 * ATOMS, V = HD * 256;
-    static constexpr int OPERANDS = 2 * Q + 2 * (K + V);
+    // a position tile's cache tiles as they are, 32 bytes apart from a multiple of 128, so that the same rows of
+    // different ones lie in different banks
+    static constexpr int RAW1 = kv4_tile_bytes(HD) + (kv4_tile_bytes(HD) % 128 ? 0 : 32), RAW = PG * RAW1;
+    static constexpr int OPERANDS = 2 * Q + 2 * (K + V) + RAW;
     // at least half an SM's shared memory: a second CTA would wait for tensor memory
     static constexpr size_t BYTES = (OPERANDS > 120 * 1024 ? OPERANDS : 120 * 1024) + 1024;
 };
 
 struct PShared {
-    unsigned long long kv_full[2], s_full[2], p_full[2], pv_done[2], fin;
+    unsigned long long kv_full[2], s_full[2], p_full[2], pv_done[2], raw_full, fin[2];
     uint32_t tmem;
     int pos[2][PG];               // first position of each cache tile of a stage
-    uint32_t nan_of[2][PN];       // groups of V that are not finite, per position
-    int nan_any[2];
-    float m[2][PM], l[2][PM], mx[2][PM];
-    uint32_t nan_row[2][PM];
+    uint8_t nan_bits[2][4][PN / 8];   // which of 8 positions' values of a group are not finite
+    alignas(16) int nan_any[2][4];    // whether an unpacking warp found any
+    float mx[2][2][PM], l[2][PM];
     int64_t part[P_THREADS / 32];
     int req, tile, found;
 };
@@ -106,7 +108,7 @@ template <int HD>
 __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq, int *flag) {
     using L = PLayout<HD>;
     constexpr int KS = HD / 16;                            // k-steps of the first product
-    constexpr uint32_t S_COL = 0, O_COL = 2 * PN;          // tensor memory: S and P of both streams, then O of both
+    constexpr uint32_t S_COL = 0, PV_COL = 2 * PN;         // tensor memory: two buffers of S and P, then two of PV
     extern __shared__ uint8_t raw[];
     __shared__ PShared sm;
     uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
@@ -164,14 +166,13 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
         for (int s = 0; s < 2; s++) {
             mbar_init(smem_u32(&sm.kv_full[s]), P_DEQ);
             mbar_init(smem_u32(&sm.s_full[s]), 1);
-            mbar_init(smem_u32(&sm.p_full[s]), P_SOFT / 2);
+            mbar_init(smem_u32(&sm.p_full[s]), P_SOFT);
             mbar_init(smem_u32(&sm.pv_done[s]), 1);
-            sm.nan_any[s] = 0;
+            mbar_init(smem_u32(&sm.fin[s]), 1);
         }
-        mbar_init(smem_u32(&sm.fin), 1);
+        mbar_init(smem_u32(&sm.raw_full), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (tid < 2 * PN) sm.nan_of[tid / PN][tid % PN] = 0;
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -194,10 +195,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                 mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[c][y].x), fabsf(x[c][y].y)), fmaxf(fabsf(x[c][y].z), fabsf(x[c][y].w))));
             }
         }
-        sm.mx[half][r] = mx;
+        sm.mx[0][half][r] = mx;
         bar_sync(1, P_SOFT);
         float up;
-        q_scales(fmaxf(sm.mx[0][r], sm.mx[1][r]), A.scale, up, kappa);
+        q_scales(fmaxf(sm.mx[0][0][r], sm.mx[0][1][r]), A.scale, up, kappa);
         kappa = fmaxf(kappa, 1e-37f);                      // -infinity * kappa stays -infinity
 #pragma unroll
         for (int c = 0; c < CH; c++) {
@@ -219,19 +220,44 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
     const uint32_t tmem = sm.tmem;
 
     if (warp < 8) {
-        // ================= softmax stream s
-        const int s = half;
+        // ================= softmax
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t t_s = tmem + lanes + S_COL + s * PN, t_o = tmem + lanes + O_COL + s * HD;
         const int i_row = i0 + r / rep, f_row = A.window && i_row >= A.window ? i_row - A.window + 1 : 0;
-        const int n = (nj - s + 1) / 2;                    // this stream's tiles
-        float m = -INFINITY, l = 0.f;
+        constexpr int OD = HD / 2, OC = OD < 32 ? 16 : 32;     // this thread's dimensions, and how many it reads at once
+        float o[OD], m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < OD; i++) o[i] = 0.f;
         uint32_t nan_mine = 0;
         bool alive = true;
-        for (int k = 0; k < n && alive; k++) {
-            alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.kv_full[s]), k & 1, flag) &&
-                                                mbar_wait(smem_u32(&sm.s_full[s]), k & 1, flag));
-            if (!alive) break;
+        // o += the PV of tile j
+        auto take = [&](int j) {
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[j & 1]), (j >> 1) & 1, flag));
+            if (!alive) return;
+            tc_fence_after();
+            const uint32_t at = tmem + lanes + PV_COL + (j & 1) * HD + half * OD;
+#pragma unroll
+            for (int c = 0; c < OD; c += OC) {
+                if constexpr (OC == 32) {
+                    uint32_t x[32];
+                    tmem_ld32(at + c, x);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[c + i] += __uint_as_float(x[i]);
+                } else {
+                    uint32_t x[16];
+                    tmem_ld16_async(at + c, x);
+                    tmem_wait_ld();
+                    tmem_regs_ready(x);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[c + i] += __uint_as_float(x[i]);
+                }
+            }
+        };
+        for (int j = 0; j < nj; j++) {
+            const int s = j & 1, k = j >> 1;
+            const uint32_t t_s = tmem + lanes + S_COL + s * PN + half * (PN / 2);
+            // (after a wait that ran out a warp goes on to meet the others at the barriers, and touches nothing)
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.kv_full[s]), k & 1, flag) &&
+                                                         mbar_wait(smem_u32(&sm.s_full[s]), k & 1, flag));
             tc_fence_after();
             // scores of 32 columns, -infinity where the row does not see the position
             auto load = [&](int c, float (&v)[32]) {
@@ -239,7 +265,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                 tmem_ld32(t_s + 32 * c, u);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int p0 = sm.pos[s][2 * c + h];
+                    const int p0 = sm.pos[s][4 * half + 2 * c + h];
                     const bool all = p0 + KV4_TILE - 1 <= i_row && (p0 >= f_row || p0 + KV4_TILE <= A.sinks);
                     if (__all_sync(0xffffffffu, all)) continue;
 #pragma unroll
@@ -251,7 +277,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             };
             float mx = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < 4; c++) {
+            for (int c = 0; c < 2 && alive; c++) {
                 float v[32];
                 load(c, v);
                 float a = v[0], b = v[1];
@@ -262,106 +288,69 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                 }
                 mx = fmaxf(mx, fmaxf(a, b));
             }
-            mx *= kappa;
-            const bool moves = mx > m + 8.f || (m == -INFINITY && mx > -INFINITY);
-            if (__any_sync(0xffffffffu, moves && m > -INFINITY)) {
-                // O in tensor memory follows; the stream's last product is done before it changes
-                alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), (k - 1) & 1, flag));
-                if (!alive) break;
-                tc_fence_after();
-                const float a = moves && m > -INFINITY ? exp2_approx(m - mx) : 1.f;
+            sm.mx[s][half][r] = mx;          // (the other buffer next time: one barrier a tile is enough)
+            bar_sync(1, P_SOFT);
+            if (!alive) continue;
+            mx = fmaxf(mx, sm.mx[s][half ^ 1][r]) * kappa;
+            const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : exp2_approx(m - mn);
+            m = mn;
+            const float ref = m == -INFINITY ? 0.f : m - 15.f;
+            float sum = 0.f;
 #pragma unroll 1
-                for (int c = 0; c < HD / 32; c++) {
-                    uint32_t o[32];
-                    tmem_ld32(t_o + 32 * c, o);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * a);
-                    tmem_st32(t_o + 32 * c, o);
-                }
-                l *= a;
-            }
-            if (moves) m = mx;
-            const float ref = m == -INFINITY ? 0.f : m - 7.f;
-#pragma unroll 1
-            for (int c = 0; c < 4; c++) {
+            for (int c = 0; c < 2; c++) {
                 float v[32];
                 load(c, v);
                 uint32_t p[32];
                 float l0 = 0.f, l1 = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float a = exp2_approx(fmaf(v[2 * i], kappa, -ref)), b = exp2_approx(fmaf(v[2 * i + 1], kappa, -ref));
-                    l0 += a;
-                    l1 += b;
-                    split2(a, b, p[i], p[16 + i]);
+                    const float x = exp2_approx(fmaf(v[2 * i], kappa, -ref)), y = exp2_approx(fmaf(v[2 * i + 1], kappa, -ref));
+                    l0 += x;
+                    l1 += y;
+                    split2(x, y, p[i], p[16 + i]);
                 }
-                l += l0 + l1;
+                sum += l0 + l1;
                 tmem_st32(t_s + 32 * c, p);
             }
-            if (sm.nan_any[s]) {                           // the same for the whole stream
+            l = fmaf(l, a, sum);
+            const int4 odd = *(const int4 *)sm.nan_any[s];
+            if (odd.x | odd.y | odd.z | odd.w) {
                 for (int i = 0; i < PN; i++) {
                     const int p = sm.pos[s][i / KV4_TILE] + i % KV4_TILE;
-                    if (p <= i_row && (p >= f_row || p < A.sinks)) nan_mine |= sm.nan_of[s][i];
+                    if (!(p <= i_row && (p >= f_row || p < A.sinks))) continue;
+                    for (int g = 0; g < HD / 32; g++) nan_mine |= (uint32_t)(sm.nan_bits[s][g][i / 8] >> (i % 8) & 1) << g;
                 }
-                bar_sync(2 + s, P_SOFT / 2);
-                sm.nan_of[s][r] = 0;
-                if (r == 0) sm.nan_any[s] = 0;
             }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(smem_u32(&sm.p_full[s]));
-        }
-        // ---- the streams join; each writes half of the dimensions
-        sm.m[s][r] = m;
-        sm.l[s][r] = l;
-        sm.nan_row[s][r] = nan_mine;
-        const int n0 = (nj + 1) / 2, n1 = nj / 2;
-        if (alive && n0 > 0) alive = mbar_wait(smem_u32(&sm.pv_done[0]), (n0 - 1) & 1, flag);
-        if (alive && n1 > 0) alive = mbar_wait(smem_u32(&sm.pv_done[1]), (n1 - 1) & 1, flag);
-        tc_fence_after();
-        bar_sync(1, P_SOFT);
-        const float m0 = sm.m[0][r], m1 = sm.m[1][r], M = fmaxf(m0, m1), top = M == -INFINITY ? 0.f : M;
-        const float a0 = exp2_approx(m0 - top), a1 = exp2_approx(m1 - top);
-        const float sum = fmaf(sm.l[0][r], a0, sm.l[1][r] * a1), inv = sum == 0.f ? 0.f : 1.f / sum;
-        const float f0 = a0 * inv, f1 = a1 * inv;
-        const uint32_t nans = sm.nan_row[0][r] | sm.nan_row[1][r];
-        float *out = A.out + (((int64_t)r_begin + t0 + r / rep) * A.n_heads + kvh * rep + r % rep) * HD;
-        const bool ok = row_ok(r);
-        constexpr int W = HD / 2 > 32 ? 32 : 16;           // dimensions at a time
-#pragma unroll 1
-        for (int d0 = s * (HD / 2); d0 < (s + 1) * (HD / 2); d0 += W) {
-            float v[W];
+            // the tile before, while this one's product runs; then both in units of the new maximum
+            if (j > 0) take(j - 1);
+            if (__any_sync(0xffffffffu, a != 1.f)) {
 #pragma unroll
-            for (int i = 0; i < W; i++) v[i] = 0.f;
-            // (all lanes take part in the loads)
-#pragma unroll
-            for (int y = 0; y < 2; y++) {
-                if ((y ? n1 : n0) == 0 || !alive) continue;
-                const uint32_t at = tmem + lanes + O_COL + y * HD + d0;
-#pragma unroll
-                for (int z = 0; z < W; z += 16) {
-                    uint32_t o[16];
-                    tmem_ld16_async(at + z, o);
-                    tmem_wait_ld();
-                    tmem_regs_ready(o);
-#pragma unroll
-                    for (int i = 0; i < 16; i++) v[z + i] = fmaf(__uint_as_float(o[i]), y ? f1 : f0, v[z + i]);
-                }
+                for (int i = 0; i < OD; i++) o[i] *= a;
             }
-            if (!ok || !alive) continue;
-            const bool bad = nans >> (d0 / 32) & 1;
+        }
+        if (alive && nj > 0) take(nj - 1);
+        sm.l[half][r] = l;
+        bar_sync(1, P_SOFT);
+        const float total = sm.l[0][r] + sm.l[1][r], inv = 1.f / total;
+        if (alive && row_ok(r)) {
+            float *out = A.out + (((int64_t)r_begin + t0 + r / rep) * A.n_heads + kvh * rep + r % rep) * HD + half * OD;
 #pragma unroll
-            for (int i = 0; i < W; i += 4)
-                *(float4 *)(out + d0 + i) = i_row < 0 || sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                            : bad ? make_float4(NAN, NAN, NAN, NAN)
-                                                  : make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            for (int i = 0; i < OD; i += 4) {
+                const bool bad = nan_mine >> ((half * OD + i) / 32) & 1;
+                *(float4 *)(out + i) = i_row < 0 || total == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                       : bad ? make_float4(NAN, NAN, NAN, NAN)
+                                             : make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+            }
         }
     } else if (warp < 12) {
         // ================= cache tiles to operands
         const int w4 = warp - 8;
         const uint32_t magic = KV4_MAGIC + (uint32_t)(A.shift >> 8);   // the shift is at most 10
         constexpr int PIECES = HD / 32, KROWS = 32 / PIECES, KI = PN / (4 * KROWS);
-        const int k_piece = lane / KROWS, k_row = w4 * KROWS + lane % KROWS;
+        const int k_piece = lane % PIECES, k_row = w4 * KROWS + lane / PIECES;
         // V: 8 positions x VW words of one 16-byte piece
         constexpr int VW = HD == 128 ? 2 : 1;
         const int vr = w4 * 4 + (lane >> 3), v_atom = vr & 1, v_chunk = (lane & 7) | (v_atom << 3);
@@ -369,6 +358,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
         const int v_word = HD == 128 ? 2 * (vr >> 3) : HD == 64 ? vr >> 2 : (vr >> 1) & 3;
         const bool v_on = HD != 32 || vr < 8;
         const int page_tiles = 1 << (A.shift - 4);
+        uint8_t *raw0 = base + 2 * L::Q + 2 * (L::K + L::V);
         // lane i < 8: where cache tile i of position tile j lies, or -1; and its first position
         auto look = [&](int j, int &pos) {
             const int u = PG * j + (lane & 7);
@@ -380,51 +370,87 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             pos = tile * KV4_TILE;
             return (int)((page * A.n_kv + kvh) * page_tiles + (tile & (page_tiles - 1)));
         };
-        uint4 kw[KI];
-        uint32_t kd[KI], vw[8][VW], vd[8];
-        int pos = ABSENT;
-        auto fetch = [&](int at) {
+        // the copies of one position tile, by the first unpacking warp
+        auto copy = [&](int at) {
+            if (w4 != 0) return;
+            const int n = __popc(__ballot_sync(0xffffffffu, lane < PG && at >= 0));
+            const uint32_t bar = smem_u32(&sm.raw_full);
+            if (lane == 0)
+                asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n}\n" ::"r"(bar),
+                             "r"(n * kv4_tile_bytes(HD))
+                             : "memory");
+            __syncwarp();
+            if (lane < PG && at >= 0)
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                 smem_u32(raw0 + lane * L::RAW1)),
+                             "l"(A.cache + (uint64_t)(uint32_t)at * kv4_tile_bytes(HD)), "r"(kv4_tile_bytes(HD)), "r"(bar)
+                             : "memory");
+        };
+        int pos = ABSENT, pos_next = ABSENT;
+        bool alive = true;
+        int at = nj > 0 ? look(0, pos) : -1, in_flight = 0;
+        if (nj > 0) {
+            copy(at);
+            in_flight = 1;
+        }
+        int at_next = nj > 1 ? look(1, pos_next) : -1;
+        for (int j = 0; j < nj; j++) {
+            const int s = j & 1;
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.raw_full), j & 1, flag));
+            in_flight = alive ? 0 : in_flight;
+            // whether every position is seen by some row (else the scales of the others count as 0)
+            const bool whole = __all_sync(0xffffffffu, lane >= PG || (at >= 0 && pos + KV4_TILE - 1 <= S.last &&
+                                                                      (pos >= S.first || pos + KV4_TILE <= A.sinks)));
+            uint4 kw[KI];
+            uint32_t kd[KI], vw[8][VW], vd[8];
 #pragma unroll
             for (int i = 0; i < KI; i++) {
-                const int row = i * 4 * KROWS + k_row, tile = __shfl_sync(0xffffffffu, at, row / KV4_TILE);
-                const int p = __shfl_sync(0xffffffffu, pos, row / KV4_TILE) + row % KV4_TILE;
-                kw[i] = make_uint4(0, 0, 0, 0);
-                kd[i] = 0;
-                if (tile >= 0 && S.any(p, A.sinks)) {
-                    const uint8_t *src = A.cache + (uint64_t)(uint32_t)tile * kv4_tile_bytes(HD);
-                    kw[i] = __ldg((const uint4 *)(src + (row % KV4_TILE) * (HD / 2) + 16 * k_piece));
-                    kd[i] = __ldg((const uint16_t *)(src + 16 * HD) + (row % KV4_TILE) * PIECES + k_piece);
-                }
+                const int row = i * 4 * KROWS + k_row, in = row % KV4_TILE;
+                const uint8_t *src = raw0 + row / KV4_TILE * L::RAW1;
+                kw[i] = *(const uint4 *)(src + in * (HD / 2) + 16 * k_piece);
+                kd[i] = *((const uint16_t *)(src + 16 * HD) + in * PIECES + k_piece);
             }
-            const int g = v_chunk >> 1, tile = __shfl_sync(0xffffffffu, at, g), p0 = __shfl_sync(0xffffffffu, pos, g) + 8 * (v_chunk & 1);
+            {
+                const uint8_t *src = raw0 + (v_chunk >> 1) * L::RAW1;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                vd[i] = 0;
-#pragma unroll
-                for (int w = 0; w < VW; w++) vw[i][w] = 0;
-                if (v_on && tile >= 0 && S.any(p0 + i, A.sinks)) {
-                    const int row = 8 * (v_chunk & 1) + i;
-                    const uint8_t *src = A.cache + (uint64_t)(uint32_t)tile * kv4_tile_bytes(HD);
-                    const uint32_t *q = (const uint32_t *)(src + 8 * HD + row * (HD / 2) + 16 * v_piece) + v_word;
+                for (int i = 0; i < 8; i++) {
+                    const int in = 8 * (v_chunk & 1) + i;
+                    const uint32_t *q = (const uint32_t *)(src + 8 * HD + in * (HD / 2) + 16 * v_piece) + v_word;
                     if constexpr (VW == 2) {
-                        const uint2 x = __ldg((const uint2 *)q);
+                        const uint2 x = *(const uint2 *)q;
                         vw[i][0] = x.x;
                         vw[i][1] = x.y;
                     } else {
-                        vw[i][0] = __ldg(q);
+                        vw[i][0] = *q;
                     }
-                    vd[i] = __ldg((const uint16_t *)(src + 17 * HD) + row * PIECES + v_piece);
+                    vd[i] = *((const uint16_t *)(src + 17 * HD) + in * PIECES + v_piece);
                 }
             }
-        };
-        int at = nj > 0 ? look(0, pos) : -1, pos_next = ABSENT;
-        int at_next = nj > 1 ? look(1, pos_next) : -1;
-        if (nj > 0) fetch(at);
-        for (int j = 0; j < nj; j++) {
-            const int s = j & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), ((j >> 1) & 1) ^ 1, flag))) break;
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < KI; i++) {
+                    const int row = i * 4 * KROWS + k_row;
+                    if (!S.any(__shfl_sync(0xffffffffu, pos, row / KV4_TILE) + row % KV4_TILE, A.sinks)) kd[i] = 0;
+                }
+                const int p0 = __shfl_sync(0xffffffffu, pos, v_chunk >> 1) + 8 * (v_chunk & 1);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (!S.any(p0 + i, A.sinks)) vd[i] = 0;
+            }
+            const int pos_here = pos;
+            bar_sync(2, P_DEQ);              // all four warps have read the raw tiles
+            if (j + 1 < nj && alive) {
+                at = at_next;
+                pos = pos_next;
+                fence_async_smem();
+                copy(at);
+                in_flight = 1;
+                at_next = j + 2 < nj ? look(j + 2, pos_next) : -1;
+            }
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), ((j >> 1) & 1) ^ 1, flag));
+            if (!alive) continue;              // (on to the next barrier of the four warps)
             uint8_t *K = base + 2 * L::Q + s * (L::K + L::V), *V = K + L::K;
-            if (w4 == 0 && lane < PG) sm.pos[s][lane] = pos;
+            if (w4 == 0 && lane < PG) sm.pos[s][lane] = pos_here;
 #pragma unroll
             for (int i = 0; i < KI; i++) {
                 const int row = i * 4 * KROWS + k_row;
@@ -438,20 +464,22 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                         make_uint4(nib_lo(w[c], d, magic), nib_lo(w8, d, magic), nib_hi(w[c], d, magic), nib_hi(w8, d, magic));
                 }
             }
-            if (v_on) {
-                uint32_t dd[4];
-                bool odd = false;
+            {
+                uint32_t odd = 0;
 #pragma unroll
-                for (int i = 0; i < 8; i++) odd = odd || not_finite(vd[i]);
+                for (int i = 0; i < 8; i++) odd |= not_finite(vd[i]) ? 1u << i : 0u;
+                if (!v_on) odd = 0;
+                if (v_on && v_word == 0) sm.nan_bits[s][v_piece][v_chunk] = (uint8_t)odd;   // one lane's per group and 8 positions
+                const int any = __any_sync(0xffffffffu, odd);
+                if (lane == 0) sm.nan_any[s][w4] = any;
                 if (odd) {
 #pragma unroll
                     for (int i = 0; i < 8; i++)
-                        if (not_finite(vd[i])) {
-                            vd[i] = 0;
-                            atomicOr(&sm.nan_of[s][8 * v_chunk + i], 1u << v_piece);
-                            sm.nan_any[s] = 1;
-                        }
+                        if (odd >> i & 1) vd[i] = 0;
                 }
+            }
+            if (v_on) {
+                uint32_t dd[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) dd[i] = __byte_perm(vd[2 * i], vd[2 * i + 1], 0x5410);
                 const uint32_t chunk = lane & 7;
@@ -477,52 +505,51 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             }
             fence_async_smem();
             mbar_arrive(smem_u32(&sm.kv_full[s]));
-            if (j + 1 < nj) {
-                at = at_next;
-                pos = pos_next;
-                fetch(at);
-                at_next = j + 2 < nj ? look(j + 2, pos_next) : -1;
-            }
+        }
+        // a copy in flight after a wait that ran out ends before the CTA does
+        if (in_flight && nj > 0) {
+            for (int phase = 0; phase < 2; phase++) mbar_wait_quiet(smem_u32(&sm.raw_full), phase);
         }
     } else if (lane == 0) {
-        // ================= MMAs
+        // ================= MMAs: warp 12 S, warp 13 PV
         constexpr uint32_t id_s = idesc_f16(PN), id_o = idesc_f16(HD);
-        auto values = [&](int j) {                         // O += P V of tile j
-            const int s = j & 1, k = j >> 1;
-            if (!mbar_wait(smem_u32(&sm.p_full[s]), k & 1, flag)) return false;
-            tc_fence_after();
-            const uint32_t v0 = kv0 + s * (L::K + L::V) + L::K, p0 = tmem + S_COL + s * PN, d = tmem + O_COL + s * HD;
+        if (warp == 12) {
+            const uint64_t qh = sw128_desc(q_hi), ql = sw128_desc(q_lo);
+            for (int j = 0; j < nj; j++) {
+                const int s = j & 1;
+                // (a stage is full only after the PV that last read this S buffer's P is done)
+                if (!mbar_wait(smem_u32(&sm.kv_full[s]), (j >> 1) & 1, flag)) break;
+                tc_fence_after();
+                const uint64_t kd = sw128_desc(kv0 + s * (L::K + L::V));
+                const uint32_t d = tmem + S_COL + s * PN;
 #pragma unroll
-            for (int ks = 0; ks < PN / 16; ks++) {
-                const uint64_t bd = sw128_desc(v0 + (ks >> 2) * (HD * 128) + (ks & 3) * 32);
-                const uint32_t a = p0 + 32 * (ks >> 1) + 8 * (ks & 1);
-                mma_ts(d, a, bd, id_o, k > 0 || ks > 0);
-                mma_ts(d, a + 16, bd, id_o, 1);
+                for (int ks = 0; ks < KS; ks++) {
+                    const uint32_t off = ((ks >> 2) * (PM * 128) + (ks & 3) * 32) >> 4;   // descriptors count 16 bytes
+                    mma_ss(d, qh + off, kd + off, id_s, ks > 0);
+                    mma_ss(d, ql + off, kd + off, id_s, 1);
+                }
+                commit(smem_u32(&sm.s_full[s]));
             }
-            commit(smem_u32(&sm.pv_done[s]));
-            return true;
-        };
-        bool alive = true;
-        for (int j = 0; j < nj && alive; j++) {
-            const int s = j & 1;
-            alive = mbar_wait(smem_u32(&sm.kv_full[s]), (j >> 1) & 1, flag);
-            if (!alive) break;
-            tc_fence_after();
-            const uint32_t k0 = kv0 + s * (L::K + L::V), d = tmem + S_COL + s * PN;
+        } else {
+            for (int j = 0; j < nj; j++) {
+                const int s = j & 1;
+                if (!mbar_wait(smem_u32(&sm.p_full[s]), (j >> 1) & 1, flag)) break;
+                tc_fence_after();
+                const uint64_t vdesc = sw128_desc(kv0 + s * (L::K + L::V) + L::K);
+                const uint32_t p0 = tmem + S_COL + s * PN, d = tmem + PV_COL + s * HD;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const uint32_t off = (ks >> 2) * (PM * 128) + (ks & 3) * 32;
-                const uint64_t bd = sw128_desc(k0 + off);
-                mma_ss(d, sw128_desc(q_hi + off), bd, id_s, ks > 0);
-                mma_ss(d, sw128_desc(q_lo + off), bd, id_s, 1);
+                for (int ks = 0; ks < PN / 16; ks++) {
+                    const uint64_t bd = vdesc + (((ks >> 2) * (HD * 128) + (ks & 3) * 32) >> 4);
+                    const uint32_t a = p0 + 32 * (ks >> 1) + 8 * (ks & 1);
+                    mma_ts(d, a, bd, id_o, ks > 0);
+                    mma_ts(d, a + 16, bd, id_o, 1);
+                }
+                commit(smem_u32(&sm.pv_done[s]));
             }
-            commit(smem_u32(&sm.s_full[s]));
-            if (j > 0) alive = values(j - 1);
         }
-        if (alive && nj > 0) alive = values(nj - 1);
         // what was issued ends before tensor memory is freed, also after a wait that ran out
-        commit(smem_u32(&sm.fin));
-        mbar_wait_quiet(smem_u32(&sm.fin), 0);
+        commit(smem_u32(&sm.fin[warp - 12]));
+        mbar_wait_quiet(smem_u32(&sm.fin[warp - 12]), 0);
     }
     tc_fence_before();
     __syncthreads();
