@@ -56,11 +56,11 @@ struct PLayout {
 };
 
 struct PShared {
-    unsigned long long kv_full[2], s_full[2], p_full[2], pv_done[2], raw_full, fin[2];
+    unsigned long long k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], raw_full, fin[2];
     uint32_t tmem;
-    int pos[2][PG];               // first position of each cache tile of a stage
-    uint8_t nan_bits[2][4][PN / 8];   // which of 8 positions' values of a group are not finite
-    alignas(16) int nan_any[2][4];    // whether an unpacking warp found any
+    int pos[4][PG];               // first position of each cache tile of a position tile (read long after K is free)
+    uint8_t nan_bits[4][4][PN / 8];   // which of 8 positions' values of a group are not finite
+    alignas(16) int nan_any[4][4];    // whether an unpacking warp found any
     float mx[2][2][PM], l[2][PM];
     int64_t part[P_THREADS / 32];
     int req, tile, found;
@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
 
     if (tid == 0) {
         for (int s = 0; s < 2; s++) {
-            mbar_init(smem_u32(&sm.kv_full[s]), P_DEQ);
+            mbar_init(smem_u32(&sm.k_full[s]), P_DEQ);
+            mbar_init(smem_u32(&sm.v_full[s]), P_DEQ);
             mbar_init(smem_u32(&sm.s_full[s]), 1);
             mbar_init(smem_u32(&sm.p_full[s]), P_SOFT);
             mbar_init(smem_u32(&sm.pv_done[s]), 1);
@@ -229,11 +230,22 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
         for (int i = 0; i < OD; i++) o[i] = 0.f;
         uint32_t nan_mine = 0;
         bool alive = true;
+        // the groups of tile j's values that are not finite, of positions that the row sees
+        auto take_nans = [&](int j) {
+            const int4 odd = *(const int4 *)sm.nan_any[j & 3];
+            if (!(odd.x | odd.y | odd.z | odd.w)) return;
+            for (int i = 0; i < PN; i++) {
+                const int p = sm.pos[j & 3][i / KV4_TILE] + i % KV4_TILE;
+                if (!(p <= i_row && (p >= f_row || p < A.sinks))) continue;
+                for (int g = 0; g < HD / 32; g++) nan_mine |= (uint32_t)(sm.nan_bits[j & 3][g][i / 8] >> (i % 8) & 1) << g;
+            }
+        };
         // o += the PV of tile j
         auto take = [&](int j) {
             alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[j & 1]), (j >> 1) & 1, flag));
             if (!alive) return;
             tc_fence_after();
+            take_nans(j);
             const uint32_t at = tmem + lanes + PV_COL + (j & 1) * HD + half * OD;
 #pragma unroll
             for (int c = 0; c < OD; c += OC) {
@@ -256,7 +268,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             const int s = j & 1, k = j >> 1;
             const uint32_t t_s = tmem + lanes + S_COL + s * PN + half * (PN / 2);
             // (after a wait that ran out a warp goes on to meet the others at the barriers, and touches nothing)
-            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.kv_full[s]), k & 1, flag) &&
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.k_full[s]), k & 1, flag) &&
                                                          mbar_wait(smem_u32(&sm.s_full[s]), k & 1, flag));
             tc_fence_after();
             // scores of 32 columns, -infinity where the row does not see the position
@@ -265,7 +277,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                 tmem_ld32(t_s + 32 * c, u);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int p0 = sm.pos[s][4 * half + 2 * c + h];
+                    const int p0 = sm.pos[j & 3][4 * half + 2 * c + h];
                     const bool all = p0 + KV4_TILE - 1 <= i_row && (p0 >= f_row || p0 + KV4_TILE <= A.sinks);
                     if (__all_sync(0xffffffffu, all)) continue;
 #pragma unroll
@@ -313,14 +325,6 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                 tmem_st32(t_s + 32 * c, p);
             }
             l = fmaf(l, a, sum);
-            const int4 odd = *(const int4 *)sm.nan_any[s];
-            if (odd.x | odd.y | odd.z | odd.w) {
-                for (int i = 0; i < PN; i++) {
-                    const int p = sm.pos[s][i / KV4_TILE] + i % KV4_TILE;
-                    if (!(p <= i_row && (p >= f_row || p < A.sinks))) continue;
-                    for (int g = 0; g < HD / 32; g++) nan_mine |= (uint32_t)(sm.nan_bits[s][g][i / 8] >> (i % 8) & 1) << g;
-                }
-            }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(smem_u32(&sm.p_full[s]));
@@ -442,15 +446,15 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             if (j + 1 < nj && alive) {
                 at = at_next;
                 pos = pos_next;
-                fence_async_smem();
                 copy(at);
                 in_flight = 1;
                 at_next = j + 2 < nj ? look(j + 2, pos_next) : -1;
             }
-            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), ((j >> 1) & 1) ^ 1, flag));
+            // K's stage is free once the S that read it is there, V's once the PV is
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.s_full[s]), ((j >> 1) & 1) ^ 1, flag));
             if (!alive) continue;              // (on to the next barrier of the four warps)
             uint8_t *K = base + 2 * L::Q + s * (L::K + L::V), *V = K + L::K;
-            if (w4 == 0 && lane < PG) sm.pos[s][lane] = pos_here;
+            if (w4 == 0 && lane < PG) sm.pos[j & 3][lane] = pos_here;
 #pragma unroll
             for (int i = 0; i < KI; i++) {
                 const int row = i * 4 * KROWS + k_row;
@@ -464,14 +468,18 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                         make_uint4(nib_lo(w[c], d, magic), nib_lo(w8, d, magic), nib_hi(w[c], d, magic), nib_hi(w8, d, magic));
                 }
             }
+            fence_async_smem();
+            mbar_arrive(smem_u32(&sm.k_full[s]));
+            alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), ((j >> 1) & 1) ^ 1, flag));
+            if (!alive) continue;
             {
                 uint32_t odd = 0;
 #pragma unroll
                 for (int i = 0; i < 8; i++) odd |= not_finite(vd[i]) ? 1u << i : 0u;
                 if (!v_on) odd = 0;
-                if (v_on && v_word == 0) sm.nan_bits[s][v_piece][v_chunk] = (uint8_t)odd;   // one lane's per group and 8 positions
+                if (v_on && v_word == 0) sm.nan_bits[j & 3][v_piece][v_chunk] = (uint8_t)odd;   // one lane's per group and 8 positions
                 const int any = __any_sync(0xffffffffu, odd);
-                if (lane == 0) sm.nan_any[s][w4] = any;
+                if (lane == 0) sm.nan_any[j & 3][w4] = any;
                 if (odd) {
 #pragma unroll
                     for (int i = 0; i < 8; i++)
@@ -504,7 +512,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                     }
             }
             fence_async_smem();
-            mbar_arrive(smem_u32(&sm.kv_full[s]));
+            mbar_arrive(smem_u32(&sm.v_full[s]));
         }
         // a copy in flight after a wait that ran out ends before the CTA does
         if (in_flight && nj > 0) {
@@ -517,8 +525,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             const uint64_t qh = sw128_desc(q_hi), ql = sw128_desc(q_lo);
             for (int j = 0; j < nj; j++) {
                 const int s = j & 1;
-                // (a stage is full only after the PV that last read this S buffer's P is done)
-                if (!mbar_wait(smem_u32(&sm.kv_full[s]), (j >> 1) & 1, flag)) break;
+                // the PV that read this buffer's P is done
+                if (!mbar_wait(smem_u32(&sm.pv_done[s]), ((j >> 1) & 1) ^ 1, flag) ||
+                    !mbar_wait(smem_u32(&sm.k_full[s]), (j >> 1) & 1, flag))
+                    break;
                 tc_fence_after();
                 const uint64_t kd = sw128_desc(kv0 + s * (L::K + L::V));
                 const uint32_t d = tmem + S_COL + s * PN;
@@ -533,7 +543,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
         } else {
             for (int j = 0; j < nj; j++) {
                 const int s = j & 1;
-                if (!mbar_wait(smem_u32(&sm.p_full[s]), (j >> 1) & 1, flag)) break;
+                if (!mbar_wait(smem_u32(&sm.v_full[s]), (j >> 1) & 1, flag) || !mbar_wait(smem_u32(&sm.p_full[s]), (j >> 1) & 1, flag)) break;
                 tc_fence_after();
                 const uint64_t vdesc = sw128_desc(kv0 + s * (L::K + L::V) + L::K);
                 const uint32_t p0 = tmem + S_COL + s * PN, d = tmem + PV_COL + s * HD;
