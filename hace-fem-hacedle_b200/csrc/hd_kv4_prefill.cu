@@ -58,7 +58,7 @@ struct PLayout {
 struct PShared {
     unsigned long long k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], raw_full, fin[2];
     uint32_t tmem;
-    int pos[4][PG];               // first position of each cache tile of a position tile (read long after K is free)
+    int pos[8][PG];               // first position of each cache tile of a position tile (read long after K is free)
     uint8_t nan_bits[4][4][PN / 8];   // which of 8 positions' values of a group are not finite
     alignas(16) int nan_any[4][4];    // whether an unpacking warp found any
     float mx[2][2][PM], l[2][PM];
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
         for (int s = 0; s < 2; s++) {
             mbar_init(smem_u32(&sm.k_full[s]), P_DEQ);
             mbar_init(smem_u32(&sm.v_full[s]), P_DEQ);
-            mbar_init(smem_u32(&sm.s_full[s]), 1);
+            mbar_init(smem_u32(&sm.s_full[s]), 2);         // the MMAs, and their issuer
             mbar_init(smem_u32(&sm.p_full[s]), P_SOFT);
             mbar_init(smem_u32(&sm.pv_done[s]), 1);
             mbar_init(smem_u32(&sm.fin[s]), 1);
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             const int4 odd = *(const int4 *)sm.nan_any[j & 3];
             if (!(odd.x | odd.y | odd.z | odd.w)) return;
             for (int i = 0; i < PN; i++) {
-                const int p = sm.pos[j & 3][i / KV4_TILE] + i % KV4_TILE;
+                const int p = sm.pos[j & 7][i / KV4_TILE] + i % KV4_TILE;
                 if (!(p <= i_row && (p >= f_row || p < A.sinks))) continue;
                 for (int g = 0; g < HD / 32; g++) nan_mine |= (uint32_t)(sm.nan_bits[j & 3][g][i / 8] >> (i % 8) & 1) << g;
             }
@@ -268,8 +268,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             const int s = j & 1, k = j >> 1;
             const uint32_t t_s = tmem + lanes + S_COL + s * PN + half * (PN / 2);
             // (after a wait that ran out a warp goes on to meet the others at the barriers, and touches nothing)
-            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.k_full[s]), k & 1, flag) &&
-                                                         mbar_wait(smem_u32(&sm.s_full[s]), k & 1, flag));
+            // k_full is not waited for here: K's stage may be filled twice before a slow warp comes by, and a parity
+            // does not tell a phase from the one after the next.  S of tile j + 2 waits for this tile's weights, so
+            // s_full cannot run ahead, and its issuer's own arrival hands on what the unpacking warps wrote.
+            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.s_full[s]), k & 1, flag));
             tc_fence_after();
             // scores of 32 columns, -infinity where the row does not see the position
             auto load = [&](int c, float (&v)[32]) {
@@ -277,7 +279,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                 tmem_ld32(t_s + 32 * c, u);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int p0 = sm.pos[j & 3][4 * half + 2 * c + h];
+                    const int p0 = sm.pos[j & 7][4 * half + 2 * c + h];
                     const bool all = p0 + KV4_TILE - 1 <= i_row && (p0 >= f_row || p0 + KV4_TILE <= A.sinks);
                     if (__all_sync(0xffffffffu, all)) continue;
 #pragma unroll
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.s_full[s]), ((j >> 1) & 1) ^ 1, flag));
             if (!alive) continue;              // (on to the next barrier of the four warps)
             uint8_t *K = base + 2 * L::Q + s * (L::K + L::V), *V = K + L::K;
-            if (w4 == 0 && lane < PG) sm.pos[j & 3][lane] = pos_here;
+            if (w4 == 0 && lane < PG) sm.pos[j & 7][lane] = pos_here;
 #pragma unroll
             for (int i = 0; i < KI; i++) {
                 const int row = i * 4 * KROWS + k_row;
@@ -539,6 +541,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                     mma_ss(d, ql + off, kd + off, id_s, 1);
                 }
                 commit(smem_u32(&sm.s_full[s]));
+                mbar_arrive(smem_u32(&sm.s_full[s]));
             }
         } else {
             for (int j = 0; j < nj; j++) {
