@@ -26,6 +26,7 @@
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
+#include <atomic>
 #include <string>
 
 #include "../../include/hacedle_cuda.h"
@@ -185,6 +186,18 @@ int hd_rope_kv_append(hd_ctx *ctx, float *qkv, int64_t ld, const int32_t *pos, i
 
 // The 4-bit cache's shape, as every entry point over it wants it (hd_kv4.cu).
 int hd_kv4_check(hd_ctx *ctx, const char *name, const void *cache, int64_t pages, int page_size, int n_kv, int head_dim);
+
+// Lets a kernel use `bytes` of dynamic shared memory (and, for clusters of
+// more than 8 CTAs, that size), once per device: `done` is the kernel's own.
+static inline cudaError_t hd_allow_smem(std::atomic<uint64_t> &done, const hd_ctx *ctx, const void *kernel, size_t bytes,
+                                        bool large_cluster = false) {
+    const uint64_t bit = (uint64_t)1 << (ctx->device & 63);
+    if (ctx->device < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && large_cluster) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
 
 // Launch with programmatic stream serialization, so the next kernel's
 // pre-dependency prologue (weight prefetch) overlaps this one's tail.

@@ -559,7 +559,8 @@ template <int HD>
 cudaError_t launch(hd_ctx *ctx, const Kv4Args &A, uint8_t *ws) {
     const int rep = A.n_heads / A.n_kv, groups = (rep + DHEADS - 1) / DHEADS, gh = (rep + groups - 1) / groups;
     const size_t smem = sizeof(DShared<HD>);
-    cudaError_t e = cudaFuncSetAttribute(k_kv4_decode<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = hd_allow_smem(allowed, ctx, (const void *)k_kv4_decode<HD>, smem);
     if (e != cudaSuccess) return e;
     // no more CTAs than the table's (or the window's) longest request can give work
     int64_t tiles = ((int64_t)A.max_pages << A.shift) / KV4_TILE;

@@ -575,7 +575,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
 template <int HD>
 cudaError_t launch(hd_ctx *ctx, const Kv4Args &A) {
     constexpr size_t smem = PLayout<HD>::BYTES;
-    cudaError_t e = cudaFuncSetAttribute(k_kv4_prefill<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = hd_allow_smem(allowed, ctx, (const void *)k_kv4_prefill<HD>, smem);
     if (e != cudaSuccess) return e;
     const int rep = A.n_heads / A.n_kv, tq = PM / rep;
     // a request's last tile may be short: at most one more tile each, and no more than rows

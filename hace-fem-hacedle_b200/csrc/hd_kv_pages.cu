@@ -233,8 +233,8 @@ extern "C" int hd_kv_pages_assign(hd_ctx *ctx, const int32_t *lens, const int32_
     if (!ctx) return HD_E_ARG;
     HdDevice on(ctx);
     const size_t smem = (size_t)(3 * reqs + 2) * sizeof(int);
-    if (smem > 48 * 1024)
-        HD_CUDA_TRY(ctx, cudaFuncSetAttribute(k_pages_assign, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<uint64_t> allowed{0};
+    HD_CUDA_TRY(ctx, hd_allow_smem(allowed, ctx, (const void *)k_pages_assign, (3 * PMAXREQ + 2) * sizeof(int)));
     // one CTA up to 2048 rows (four a thread), then one more for each 2048, eight at most
     const int64_t want = (max_rows + 4 * PNT - 1) / (4 * PNT);
     const int ctas = want < 1 ? 1 : want > 8 ? 8 : (int)want;

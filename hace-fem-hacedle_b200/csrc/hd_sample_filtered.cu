@@ -49,6 +49,7 @@ namespace {
 constexpr int FBINS = 1024, FGROUP = 16, FGROUPS = FBINS / FGROUP;   // FGROUPS: also the first histogram's bins
 constexpr int CANDS = 2048;                  // elements of the first histogram's bin that a slice lists
 constexpr int CAP = 512;                     // elements compared with one another
+constexpr int64_t FULL = 46080;              // elements of a slice that shared memory holds at most
 constexpr int MAXC = 16;                     // CTAs per row
 constexpr int MAXW = 32;                     // warps per CTA
 constexpr uint32_t KEY_NINF = 0x007fffffu;   // key of -infinity
@@ -775,8 +776,8 @@ cudaError_t launch(hd_ctx *ctx, int C, int64_t rows, int64_t slice, const float 
                    double unit, int half, int32_t *idx) {
     const size_t smem = (sizeof(FShared) + 15) / 16 * 16 + (RESIDENT ? (size_t)slice * sizeof(float) : 0);
     auto kernel = k_sample_filtered<NT, RESIDENT>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = hd_allow_smem(allowed, ctx, (const void *)kernel, sizeof(FShared) + 16 + (RESIDENT ? FULL * sizeof(float) : 0), true);
     if (e != cudaSuccess) return e;
     const int wide = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
     return hd_launch_cluster(ctx, kernel, dim3((unsigned)(rows * C)), dim3(NT), smem, C, logits, ld, n, temperature, top_k,
@@ -798,7 +799,7 @@ extern "C" int hd_sample_filtered(hd_ctx *ctx, const float *logits, int64_t ld, 
     HdDevice on(ctx);
     // CTAs per row: as few as keep a slice at 80 KB, so that two CTAs share an SM; more while the rows
     // alone leave SMs idle and a slice keeps 2048 elements
-    constexpr int64_t HALF = FS_HALF, FULL = 49152;
+    constexpr int64_t HALF = FS_HALF;
     auto slice_of = [&](int c) { return ((n + c - 1) / c + 3) / 4 * 4; };
     int C = 1;
     while (C < MAXC && (slice_of(C) > HALF || (rows * C < ctx->sm_count && slice_of(C) > 4096))) C *= 2;

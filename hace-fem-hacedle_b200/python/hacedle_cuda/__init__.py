@@ -138,23 +138,34 @@ def _ptr(t) -> int | None:
     return t.data_ptr()
 
 
-def _f32_rows(t, name: str) -> int:
-    """Row stride of a float32 tensor whose rows are dense."""
+# The paged-cache and sampling calls are short on the GPU, so their checks are
+# kept to what a wrong tensor could break: type, density and size.
+_I32 = _F32 = _U8 = None
+
+
+def _dtypes():
+    global _I32, _F32, _U8
     import torch
 
-    if t.dtype != torch.float32 or t[0].numel() > 1 and not t[0].is_contiguous():
-        raise ValueError(f"{name} must be float32 with dense rows")
-    return t.stride(0)
+    _I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 
 
-def _dense(dtype_name: str, **tensors):
-    """Every given tensor is dense and of the dtype."""
-    import torch
+def _dense(dtype, *tensors):
+    for t in tensors:
+        if t.dtype is not dtype or not t.is_contiguous():
+            raise ValueError(f"a dense {dtype} tensor is wanted, not {t.dtype} of strides {t.stride()}")
 
-    dtype = getattr(torch, dtype_name)
-    for name, t in tensors.items():
-        if t is not None and (t.dtype != dtype or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a dense {dtype_name} tensor")
+
+def _row_stride(t) -> int:
+    """Row stride of a float32 tensor [rows, ...] whose rows are dense (0: all of it is)."""
+    if t.dtype is not _F32:
+        raise ValueError(f"a float32 tensor is wanted, not {t.dtype}")
+    if t.is_contiguous() or t.shape[0] < 2 and t[:1].is_contiguous():
+        return 0
+    ld = t.stride(0)
+    if not t[0].is_contiguous() or ld < t[0].numel():
+        raise ValueError(f"rows must be dense and apart, not of strides {t.stride()}")
+    return ld
 
 
 def kv4_cache_shape(pages: int, page_size: int, n_kv: int, head_dim: int) -> tuple[int, int, int, int]:
@@ -266,14 +277,25 @@ class Context:
         """One int32 index per row of float32 logits [rows, n] (rows may be
         strided) from u [rows] in [0, 1), after temperature, top-k, top-p and
         min-p; the settings are [rows] tensors (top_k int32) or None."""
-        _dense("float32", u=u, temperature=temperature, top_p=top_p, min_p=min_p)
-        _dense("int32", idx=idx, top_k=top_k)
+        if _I32 is None:
+            _dtypes()
         rows, n = logits.shape
-        if any(t is not None and t.numel() != rows for t in (u, idx, temperature, top_k, top_p, min_p)):
+        _dense(_F32, u)
+        _dense(_I32, idx)
+        bad = u.numel() != rows or idx.numel() != rows
+        for t in (temperature, top_p, min_p):
+            if t is not None:
+                _dense(_F32, t)
+                bad = bad or t.numel() != rows
+        if top_k is not None:
+            _dense(_I32, top_k)
+            bad = bad or top_k.numel() != rows
+        if bad:
             raise ValueError(f"u, idx and the settings must have one entry for each of the {rows} rows")
-        ld = _f32_rows(logits, "logits") if rows else n
-        self._check(lib().hd_sample_filtered(self.h, _ptr(logits), ld if rows > 1 else n, rows, n, _ptr(temperature),
-                                             _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(u), _ptr(idx)))
+        rc = lib().hd_sample_filtered(self.h, logits.data_ptr(), _row_stride(logits), rows, n, _ptr(temperature), _ptr(top_k),
+                                      _ptr(top_p), _ptr(min_p), u.data_ptr(), idx.data_ptr())
+        if rc:
+            self._check(rc)
 
     # ---- paged KV cache ----
     def kv_pages_assign(self, lens, new, tables, page_size: int, pages: int, free, n_free, n_free_out, lens_out, row0, slots,
@@ -281,29 +303,37 @@ class Context:
         """Places new[r] tokens of each request (hd_kv_pages_assign); every
         argument an int32 device tensor, tables [reqs, max_pages], slots and
         pos [max_rows]; n_free_out / lens_out may be n_free / lens."""
-        _dense("int32", lens=lens, new=new, tables=tables, free=free, n_free=n_free, n_free_out=n_free_out, lens_out=lens_out,
-               row0=row0, slots=slots, pos=pos, status=status)
+        if _I32 is None:
+            _dtypes()
+        _dense(_I32, lens, new, tables, free, n_free, n_free_out, lens_out, row0, slots, pos, status)
         reqs, width = tables.shape
+        rows = slots.numel()
         if lens.numel() != reqs or new.numel() != reqs or lens_out.numel() != reqs or row0.numel() != reqs + 1 or \
-                slots.numel() != pos.numel():
+                rows != pos.numel():
             raise ValueError(f"lens, new, lens_out, row0, slots or pos do not fit {reqs} requests")
-        self._check(lib().hd_kv_pages_assign(self.h, _ptr(lens), _ptr(new), reqs, _ptr(tables), width, page_size, pages,
-                                             _ptr(free), _ptr(n_free), _ptr(n_free_out), _ptr(lens_out), _ptr(row0),
-                                             _ptr(slots), _ptr(pos), slots.numel(), _ptr(status)))
+        rc = lib().hd_kv_pages_assign(self.h, lens.data_ptr(), new.data_ptr(), reqs, tables.data_ptr(), width, page_size, pages,
+                                      free.data_ptr(), n_free.data_ptr(), n_free_out.data_ptr(), lens_out.data_ptr(),
+                                      row0.data_ptr(), slots.data_ptr(), pos.data_ptr(), rows, status.data_ptr())
+        if rc:
+            self._check(rc)
 
     def kv_pages_release(self, done, lens, tables, page_size: int, free, n_free, status):
         """Gives back the pages of the requests with done[r] != 0."""
-        _dense("int32", done=done, lens=lens, tables=tables, free=free, n_free=n_free, status=status)
+        if _I32 is None:
+            _dtypes()
+        _dense(_I32, done, lens, tables, free, n_free, status)
         reqs, width = tables.shape
         if lens.numel() != reqs or done.numel() != reqs:
             raise ValueError(f"lens or done do not fit {reqs} requests")
-        self._check(lib().hd_kv_pages_release(self.h, _ptr(done), _ptr(lens), reqs, _ptr(tables), width, page_size, _ptr(free),
-                                              _ptr(n_free), free.numel(), _ptr(status)))
+        self._check(lib().hd_kv_pages_release(self.h, done.data_ptr(), lens.data_ptr(), reqs, tables.data_ptr(), width,
+                                              page_size, free.data_ptr(), n_free.data_ptr(), free.numel(), status.data_ptr()))
 
     @staticmethod
     def _kv4_shape(cache):
         """(pages, page_size, n_kv, head_dim) of a uint8 cache tensor [pages, n_kv, page_size / 16, 18 * head_dim]."""
-        _dense("uint8", cache=cache)
+        if _I32 is None:
+            _dtypes()
+        _dense(_U8, cache)
         if cache.dim() != 4 or cache.shape[3] % 18:
             raise ValueError("cache must be [pages, n_kv, page_size / 16, 18 * head_dim]")
         pages, n_kv, tiles, width = cache.shape
@@ -312,60 +342,78 @@ class Context:
     def kv4_append(self, k, v, slots, cache):
         """k, v [rows, n_kv, head_dim] (rows may be strided) quantized into the cache's slots."""
         pages, page, n_kv, hd = self._kv4_shape(cache)
+        _dense(_I32, slots)
         rows = slots.numel()
-        _dense("int32", slots=slots)
-        if k.shape[0] != rows or v.shape[0] != rows or k.numel() != rows * n_kv * hd or v.numel() != k.numel():
+        n = rows * n_kv * hd
+        if k.shape[0] != rows or v.shape[0] != rows or k.numel() != n or v.numel() != n:
             raise ValueError("k, v, slots and cache do not fit")
-        if rows:
-            self._check(lib().hd_kv4_append(self.h, _ptr(k), _ptr(v), _f32_rows(k, "k") if rows > 1 else 0,
-                                            _f32_rows(v, "v") if rows > 1 else 0, _ptr(slots), rows, n_kv, hd, _ptr(cache),
-                                            pages, page))
+        rc = lib().hd_kv4_append(self.h, k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v), slots.data_ptr(), rows,
+                                 n_kv, hd, cache.data_ptr(), pages, page)
+        if rc:
+            self._check(rc)
 
     def kv4_read(self, cache, slots, k, v):
         """The values that slots hold into k, v [rows, n_kv, head_dim]."""
         pages, page, n_kv, hd = self._kv4_shape(cache)
-        _dense("int32", slots=slots)
-        _dense("float32", k=k, v=v)
-        if k.numel() != slots.numel() * n_kv * hd or v.numel() != k.numel():
+        _dense(_I32, slots)
+        _dense(_F32, k, v)
+        rows = slots.numel()
+        n = rows * n_kv * hd
+        if k.numel() != n or v.numel() != n:
             raise ValueError("k, v, slots and cache do not fit")
-        self._check(lib().hd_kv4_read(self.h, _ptr(cache), pages, page, _ptr(slots), slots.numel(), n_kv, hd, _ptr(k),
-                                      _ptr(v)))
+        rc = lib().hd_kv4_read(self.h, cache.data_ptr(), pages, page, slots.data_ptr(), rows, n_kv, hd, k.data_ptr(),
+                               v.data_ptr())
+        if rc:
+            self._check(rc)
 
     def kv4_workspace_bytes(self, n_heads: int, n_kv: int, head_dim: int) -> int:
         return int(lib().hd_kv4_workspace_bytes(self.h, n_heads, n_kv, head_dim))
 
-    def _kv4_rows(self, q, cache, tables, lens, out, n_lens):
-        shape = self._kv4_shape(cache)
-        _dense("int32", tables=tables, lens=lens)
-        _dense("float32", out=out)
-        if tables.dim() != 2 or tables.shape[0] != n_lens or lens.numel() != n_lens or out.numel() != q.numel() or \
-                q.numel() % (max(1, q.shape[0]) * shape[3]):
+    @staticmethod
+    def _kv4_heads(q, tables, lens, out, hd: int) -> int:
+        _dense(_I32, tables, lens)
+        _dense(_F32, out)
+        rows, n = q.shape[0], q.numel()
+        heads = n // (rows * hd)
+        if tables.dim() != 2 or tables.shape[0] != lens.numel() or out.numel() != n or heads * rows * hd != n:
             raise ValueError("q, cache, tables, lens and out do not fit")
-        heads = q.numel() // max(1, q.shape[0]) // shape[3]
-        return shape, heads, _f32_rows(q, "q") if q.shape[0] > 1 else 0
+        return heads
 
     def kv4_attention_decode(self, q, cache, tables, lens, out, window: int = 0, sinks: int = 0, scale: float = 0.0, ws=None):
         """q [seqs, heads, head_dim] (rows may be strided): each request's last
         position against its cached ones.  ws: a zeroed uint8 tensor of
         kv4_workspace_bytes, or None for the context's own."""
-        if not q.shape[0]:
+        pages, page, n_kv, hd = self._kv4_shape(cache)
+        seqs = lens.numel()
+        if q.shape[0] != seqs:
+            raise ValueError("q must have one row for each request")
+        if not seqs:
             return
-        (pages, page, n_kv, hd), heads, ld = self._kv4_rows(q, cache, tables, lens, out, q.shape[0])
-        self._check(lib().hd_kv4_attention_decode(self.h, _ptr(q), ld, _ptr(cache), pages, page, _ptr(tables), tables.shape[1],
-                                                  _ptr(lens), lens.numel(), heads, n_kv, hd, window, sinks, scale, _ptr(out),
-                                                  _ptr(ws), ws.numel() if ws is not None else 0))
+        heads = self._kv4_heads(q, tables, lens, out, hd)
+        if ws is not None:
+            _dense(_U8, ws)
+        rc = lib().hd_kv4_attention_decode(self.h, q.data_ptr(), _row_stride(q), cache.data_ptr(), pages, page,
+                                           tables.data_ptr(), tables.shape[1], lens.data_ptr(), seqs, heads, n_kv, hd, window,
+                                           sinks, scale, out.data_ptr(), None if ws is None else ws.data_ptr(),
+                                           0 if ws is None else ws.numel())
+        if rc:
+            self._check(rc)
 
     def kv4_attention_prefill(self, q, cache, tables, lens, row0, out, window: int = 0, sinks: int = 0, scale: float = 0.0):
         """q [rows, heads, head_dim]: rows row0[r] .. row0[r+1]-1 are request r's last positions."""
-        if not q.shape[0]:
+        pages, page, n_kv, hd = self._kv4_shape(cache)
+        rows, seqs = q.shape[0], lens.numel()
+        if not rows:
             return
-        (pages, page, n_kv, hd), heads, ld = self._kv4_rows(q, cache, tables, lens, out, lens.numel())
-        _dense("int32", row0=row0)
-        if row0.numel() != lens.numel() + 1:
+        heads = self._kv4_heads(q, tables, lens, out, hd)
+        _dense(_I32, row0)
+        if row0.numel() != seqs + 1:
             raise ValueError("row0 must have one more entry than lens")
-        self._check(lib().hd_kv4_attention_prefill(self.h, _ptr(q), ld, _ptr(cache), pages, page, _ptr(tables),
-                                                   tables.shape[1], _ptr(lens), _ptr(row0), lens.numel(), q.shape[0], heads,
-                                                   n_kv, hd, window, sinks, scale, _ptr(out)))
+        rc = lib().hd_kv4_attention_prefill(self.h, q.data_ptr(), _row_stride(q), cache.data_ptr(), pages, page,
+                                            tables.data_ptr(), tables.shape[1], lens.data_ptr(), row0.data_ptr(), seqs, rows,
+                                            heads, n_kv, hd, window, sinks, scale, out.data_ptr())
+        if rc:
+            self._check(rc)
 
     def dequantize(self, w: Weight, out):
         self._check(lib().hd_dequantize(self.h, w.h, _ptr(out), out.numel()))

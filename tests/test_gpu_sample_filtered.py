@@ -1,8 +1,8 @@
 """Filtered sampling against the 64-bit model: equal indices wherever no
 decision lies so close to its border that the weights' rounding could cross it.
 
-A weight is rounded to a multiple of 2^-s of the largest, s at least 40 (more
-for rows of less than 786432), so it is off by at most 2^-41, and the sums are
+A weight is rounded to a multiple of 2^-s of the largest, s at least 40 (for
+rows that a cluster holds), so it is off by at most 2^-41, and the sums are
 exact; the n roundings are independent, each of standard deviation 2^-40 / sqrt(12), so a
 running sum is off by 6 sqrt(n) 2^-40 / sqrt(12) at six standard deviations,
 against a mass of at least 1; a weight itself is computed to 2^-48 of itself.  The model's own sums in 64 bits add n 2^-53 of the mass at most."""

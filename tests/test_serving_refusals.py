@@ -113,6 +113,9 @@ def test_the_binding_refuses_tensors_that_do_not_fit():
         lambda: ctx.kv4_attention_prefill(q, cache, i32(2, 4), i32(2), i32(2), out),
         lambda: ctx.sample_filtered(torch.zeros(2, 50), torch.zeros(3), i32(2)),
         lambda: ctx.sample_filtered(torch.zeros(2, 50), torch.zeros(2), i32(2), top_k=torch.zeros(2)),
+        lambda: ctx.kv4_attention_decode(q[:1].expand(3, 4, 64), cache, i32(3, 4), i32(3), out),
+        lambda: ctx.kv4_append(torch.zeros(1, 2, 64).expand(4, 2, 64), torch.zeros(4, 2, 64), i32(4), cache),
+        lambda: ctx.sample_filtered(torch.zeros(1, 50).expand(2, 50), torch.zeros(2), i32(2)),
         lambda: ctx.sample_filtered(torch.zeros(50, 2).t(), torch.zeros(2), i32(2)),
         lambda: ctx.kv_pages_assign(i32(2), i32(2), i32(3, 4), 16, 8, i32(8), i32(1), i32(1), i32(3), i32(4), i32(5), i32(5), i32(1)),
         lambda: ctx.kv_pages_release(i32(2), i32(3), i32(3, 4), 16, i32(8), i32(1), i32(1)),
