@@ -282,14 +282,16 @@ __device__ __noinline__ void part(FShared &sm, int b, int e, float ft) {
     }
 }
 
-// f(rank) summed over the cluster, every load in flight at once.
+// f(rank) summed over the cluster, four loads in flight at a time.
 template <typename F>
 __device__ __forceinline__ long long cluster_sum(unsigned C, F f) {
     long long v = 0;
+    for (unsigned r = 0; r < C; r += 4) {
+        long long x[4];
 #pragma unroll
-    for (unsigned r = 0; r < MAXC; r++) {
-        const long long x = f(r < C ? r : 0);
-        v += r < C ? x : 0;
+        for (unsigned i = 0; i < 4; i++) x[i] = f(r + i < C ? r + i : r);
+#pragma unroll
+        for (unsigned i = 0; i < 4; i++) v += r + i < C ? x[i] : 0;
     }
     return v;
 }
@@ -317,11 +319,13 @@ __device__ uint32_t last_key(uint32_t top, F low) {
 // (and of floor_ties of those equal to it), from the largest down, reaches its
 // goal: `goal` of them, or (MASS) the share p of their units.  `above`: the
 // weight of the elements > tau.  Every CTA of the cluster gets the same.
+// `few`: the elements above the floor are at most CAP together (top-k has
+// left them): they are listed at once and compared, without a histogram.
 // `own` becomes the slice's own weight above tau and its elements equal to it
 // where the histogram tells (MASS, one level), and -1 elsewhere.
 template <int NT, bool RESIDENT, bool MASS>
-__device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long long floor_ties, double p, long long &goal,
-                           long long &above, long long &own, int &own_ties) {
+__device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long long floor_ties, bool few, double p,
+                           long long &goal, long long &above, long long &own, int &own_ties) {
     constexpr int NW = NT / 32;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -352,145 +356,152 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
         }
     };
     for (int level = 0;; level++) {
-        if (level == 0)
-            for (int b = tid; b < FGROUPS * 32; b += NT) sm.lane_lo[b] = sm.lane_hi[b] = 0;
-        else
-            for (int b = tid; b < FBINS; b += NT) sm.lo[b] = sm.hi[b] = 0;
-        if (tid == 0) sm.n_list = 0;
-        __syncthreads();
-        if (level == 0) {
-            first_histogram<NT, RESIDENT, MASS>(sm, key_value(lo_key));
+        int pick = 0;
+        uint32_t kl_list = lo_key, kh = hi_key;
+        if (few) {
+            if (tid == 0) sm.n_list = 0;
+            __syncthreads();
         } else {
-            auto count = [&](uint32_t key) {
-                if (key < lo_key || key > hi_key) return;
-                const int b = (int)((hi_key - key) >> shift);
-                if (!MASS) {
-                    atomicAdd(&sm.lo[b], 1u);
-                } else {
-                    add64(sm.lo, sm.hi, b, (unsigned long long)R.units(key_value(key)));
-                }
-            };
-            each(count);
-        }
-        __syncthreads();
-        // groups of 16 bins, or the first histogram's bins of 32 lanes: eight threads each
-        for (int q = tid / 8; q < FGROUPS; q += NT / 8) {
-            unsigned long long s = 0;
+            if (level == 0)
+                for (int b = tid; b < FGROUPS * 32; b += NT) sm.lane_lo[b] = sm.lane_hi[b] = 0;
+            else
+                for (int b = tid; b < FBINS; b += NT) sm.lo[b] = sm.hi[b] = 0;
+            if (tid == 0) sm.n_list = 0;
+            __syncthreads();
             if (level == 0) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int b = q * 32 + 4 * (tid & 7) + i;
-                    s += ((unsigned long long)sm.lane_hi[b] << (RESIDENT ? R.half : 32)) + sm.lane_lo[b];
-                }
+                first_histogram<NT, RESIDENT, MASS>(sm, key_value(lo_key));
             } else {
+                auto count = [&](uint32_t key) {
+                    if (key < lo_key || key > hi_key) return;
+                    const int b = (int)((hi_key - key) >> shift);
+                    if (!MASS) {
+                        atomicAdd(&sm.lo[b], 1u);
+                    } else {
+                        add64(sm.lo, sm.hi, b, (unsigned long long)R.units(key_value(key)));
+                    }
+                };
+                each(count);
+            }
+            __syncthreads();
+            // groups of 16 bins, or the first histogram's bins of 32 lanes: eight threads each
+            for (int q = tid / 8; q < FGROUPS; q += NT / 8) {
+                unsigned long long s = 0;
+                if (level == 0) {
 #pragma unroll
-                for (int i = 0; i < FGROUP / 8; i++) {
-                    const int b = q * FGROUP + FGROUP / 8 * (tid & 7) + i;
-                    s += ((unsigned long long)sm.hi[b] << 32) + sm.lo[b];
-                }
-            }
+                    for (int i = 0; i < 4; i++) {
+                        const int b = q * 32 + 4 * (tid & 7) + i;
+                        s += ((unsigned long long)sm.lane_hi[b] << (RESIDENT ? R.half : 32)) + sm.lane_lo[b];
+                    }
+                } else {
 #pragma unroll
-            for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if ((tid & 7) == 0) sm.group[q] = (long long)s;
-        }
-        cluster.sync();
-        const int floor_bin = !with_floor ? -1 : level == 0 ? R.bin(key_value(floor_key)) * FGROUP : (int)((hi_key - floor_key) >> shift);
-        if (tid < FGROUPS)
-            sm.total[tid] = (floor_bin >= 0 && floor_bin / FGROUP == tid ? floor_w : 0) +
-                            cluster_sum(C, [&](unsigned r) { return cluster.map_shared_rank(&sm, r)->group[tid]; });
-        __syncthreads();
-        if (warp == 0) {
-            const long long t0 = sm.total[2 * lane], t1 = sm.total[2 * lane + 1];
-            const long long inc = warp_scan(t0 + t1);
-            if (MASS && level == 0) {
-                const long long mass = __shfl_sync(0xffffffffu, inc, 31);
-                goal = __double2ll_ru(p * (double)mass);
-                goal = goal < 1 ? 1 : goal > mass ? mass : goal;
-            }
-            const long long b0 = above + inc - t0 - t1, b1 = b0 + t0, b2 = b1 + t1;
-            const bool mine = b0 < goal && b2 >= goal;
-            const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
-            const int q = __shfl_sync(0xffffffffu, b1 >= goal ? 2 * lane : 2 * lane + 1, src);
-            const long long base = __shfl_sync(0xffffffffu, b1 >= goal ? b0 : b1, src);
-            if (lane == 0) {
-                sm.bin = q;
-                sm.bin_above = base;
-                sm.goal = goal;
-            }
-        }
-        __syncthreads();
-        goal = sm.goal;
-        if (level > 0) {
-            // the group's bins: a warp per CTA fetches them, one adds them up
-            const int q = sm.bin;
-            if (warp < (int)C && lane < FGROUP) {
-                const FShared *o = cluster.map_shared_rank(&sm, warp);
-                sm.part[warp][lane] = (long long)(((unsigned long long)o->hi[q * FGROUP + lane] << 32) | o->lo[q * FGROUP + lane]);
-            }
-            __syncthreads();
-            if (warp == 0) {
-                const int b = q * FGROUP + lane;
-                long long v = lane < FGROUP && floor_bin == b ? floor_w : 0;
-                if (lane < FGROUP)
-                    for (unsigned r = 0; r < C; r++) v += sm.part[r][lane];
-                const long long run = sm.bin_above + warp_scan(v);
-                const int first = __ffs(__ballot_sync(0xffffffffu, run >= goal)) - 1;
-                __syncwarp();
-                if (lane == first) {
-                    sm.bin = b;
-                    sm.bin_above = run - v;
+                    for (int i = 0; i < FGROUP / 8; i++) {
+                        const int b = q * FGROUP + FGROUP / 8 * (tid & 7) + i;
+                        s += ((unsigned long long)sm.hi[b] << 32) + sm.lo[b];
+                    }
                 }
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if ((tid & 7) == 0) sm.group[q] = (long long)s;
             }
-            __syncthreads();
-        }
-        const int pick = sm.bin;
-        above = sm.bin_above;
-        // the bin's keys
-        uint32_t kl, kh;
-        if (level == 0) {
-            if (warp < 2) {
-                const int v = pick + warp;   // the largest key of a bin >= v
-                const uint32_t k = v == 0 ? order_key(R.top) : v >= FGROUPS ? KEY_NINF - 1 : last_key(order_key(R.top), [&](uint32_t c) { return R.bin(key_value(c)) >= v; });
-                if (lane == 0) sm.bound[warp] = k;
-            }
-            __syncthreads();
-            kl = max(lo_key, sm.bound[1] + 1);
-            kh = sm.bound[0];
-        } else {
-            kh = hi_key - ((uint32_t)pick << shift);
-            const uint32_t width = (1u << shift) - 1;
-            kl = kh - lo_key < width ? lo_key : kh - width;
-        }
-        with_floor = with_floor && (level == 0 ? floor_bin / FGROUP : floor_bin) == pick;
-        if (with_floor) kl = floor_key;      // the floor's own below the others
-        if (kl == kh) {
-            cluster.sync();                  // before the histogram is written again
-            return kl;
-        }
-        if (level == 0) {
-            if (MASS)
-                for (int q = 0; q < pick; q++) own_above += sm.group[q];
-            lo_key = with_floor ? floor_key + 1 : kl;
-            hi_key = kh;
-            shift = 0;
-            while ((hi_key - kl) >> shift >= FBINS) shift++;
-            // list the bin's elements, over the histogram: its sums are in group, which nobody reads any more
-            // from here on but this CTA
-            if (tid == 0) sm.n_cand = 0;
-            __syncthreads();
-            list_bin<NT, RESIDENT>(sm, key_value(lo_key), key_value(hi_key));
             cluster.sync();
-            // by a warp, for all
+            const int floor_bin = !with_floor ? -1 : level == 0 ? R.bin(key_value(floor_key)) * FGROUP : (int)((hi_key - floor_key) >> shift);
+            if (tid < FGROUPS)
+                sm.total[tid] = (floor_bin >= 0 && floor_bin / FGROUP == tid ? floor_w : 0) +
+                                cluster_sum(C, [&](unsigned r) { return cluster.map_shared_rank(&sm, r)->group[tid]; });
+            __syncthreads();
             if (warp == 0) {
-                const uint32_t c = cluster.map_shared_rank(&sm, lane < (int)C ? lane : 0)->n_cand;
-                const int ok = __all_sync(0xffffffffu, c <= CANDS);
-                if (lane == 0) sm.found = ok;
+                const long long t0 = sm.total[2 * lane], t1 = sm.total[2 * lane + 1];
+                const long long inc = warp_scan(t0 + t1);
+                if (MASS && level == 0) {
+                    const long long mass = __shfl_sync(0xffffffffu, inc, 31);
+                    goal = __double2ll_ru(p * (double)mass);
+                    goal = goal < 1 ? 1 : goal > mass ? mass : goal;
+                }
+                const long long b0 = above + inc - t0 - t1, b1 = b0 + t0, b2 = b1 + t1;
+                const bool mine = b0 < goal && b2 >= goal;
+                const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+                const int q = __shfl_sync(0xffffffffu, b1 >= goal ? 2 * lane : 2 * lane + 1, src);
+                const long long base = __shfl_sync(0xffffffffu, b1 >= goal ? b0 : b1, src);
+                if (lane == 0) {
+                    sm.bin = q;
+                    sm.bin_above = base;
+                    sm.goal = goal;
+                }
             }
             __syncthreads();
-            listed = sm.found;
-            continue;
+            goal = sm.goal;
+            if (level > 0) {
+                // the group's bins: a warp per CTA fetches them, one adds them up
+                const int q = sm.bin;
+                if (warp < (int)C && lane < FGROUP) {
+                    const FShared *o = cluster.map_shared_rank(&sm, warp);
+                    sm.part[warp][lane] = (long long)(((unsigned long long)o->hi[q * FGROUP + lane] << 32) | o->lo[q * FGROUP + lane]);
+                }
+                __syncthreads();
+                if (warp == 0) {
+                    const int b = q * FGROUP + lane;
+                    long long v = lane < FGROUP && floor_bin == b ? floor_w : 0;
+                    if (lane < FGROUP)
+                        for (unsigned r = 0; r < C; r++) v += sm.part[r][lane];
+                    const long long run = sm.bin_above + warp_scan(v);
+                    const int first = __ffs(__ballot_sync(0xffffffffu, run >= goal)) - 1;
+                    __syncwarp();
+                    if (lane == first) {
+                        sm.bin = b;
+                        sm.bin_above = run - v;
+                    }
+                }
+                __syncthreads();
+            }
+            pick = sm.bin;
+            above = sm.bin_above;
+            // the bin's keys
+            uint32_t kl;
+            if (level == 0) {
+                if (warp < 2) {
+                    const int v = pick + warp;   // the largest key of a bin >= v
+                    const uint32_t k = v == 0 ? order_key(R.top) : v >= FGROUPS ? KEY_NINF - 1 : last_key(order_key(R.top), [&](uint32_t c) { return R.bin(key_value(c)) >= v; });
+                    if (lane == 0) sm.bound[warp] = k;
+                }
+                __syncthreads();
+                kl = max(lo_key, sm.bound[1] + 1);
+                kh = sm.bound[0];
+            } else {
+                kh = hi_key - ((uint32_t)pick << shift);
+                const uint32_t width = (1u << shift) - 1;
+                kl = kh - lo_key < width ? lo_key : kh - width;
+            }
+            with_floor = with_floor && (level == 0 ? floor_bin / FGROUP : floor_bin) == pick;
+            if (with_floor) kl = floor_key;      // the floor's own below the others
+            if (kl == kh) {
+                cluster.sync();                  // before the histogram is written again
+                return kl;
+            }
+            if (level == 0) {
+                if (MASS)
+                    for (int q = 0; q < pick; q++) own_above += sm.group[q];
+                lo_key = with_floor ? floor_key + 1 : kl;
+                hi_key = kh;
+                shift = 0;
+                while ((hi_key - kl) >> shift >= FBINS) shift++;
+                // list the bin's elements, over the histogram: its sums are in group, which nobody reads any more
+                // from here on but this CTA
+                if (tid == 0) sm.n_cand = 0;
+                __syncthreads();
+                list_bin<NT, RESIDENT>(sm, key_value(lo_key), key_value(hi_key));
+                cluster.sync();
+                // by a warp, for all
+                if (warp == 0) {
+                    const uint32_t c = cluster.map_shared_rank(&sm, lane < (int)C ? lane : 0)->n_cand;
+                    const int ok = __all_sync(0xffffffffu, c <= CANDS);
+                    if (lane == 0) sm.found = ok;
+                }
+                __syncthreads();
+                listed = sm.found;
+                continue;
+            }
+            kl_list = with_floor ? floor_key + 1 : kl;
         }
-        const uint32_t kl_list = with_floor ? floor_key + 1 : kl;
         auto put = [&](uint32_t key) {
             if (key < kl_list || key > kh) return;
             const uint32_t at = atomicAdd(&sm.n_list, 1u);
@@ -521,6 +532,19 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
             for (int i = tid; i < L; i += NT)
                 sm.weight[i] = i == (int)all ? floor_w : MASS ? R.units(key_value(sm.all[i])) : 1;
             __syncthreads();
+            if (few) {                       // their mass is known only now
+                if (warp == 0) {
+                    long long mass = 0;
+                    for (int i = lane; i < L; i += 32) mass += sm.weight[i];
+                    mass = warp_sum(mass);
+                    if (lane == 0) {
+                        const long long to = __double2ll_ru(p * (double)mass);
+                        sm.goal = to < 1 ? 1 : to > mass ? mass : to;
+                    }
+                }
+                __syncthreads();
+                goal = sm.goal;
+            }
             // every CTA compares its share of the elements with all of them, half a warp an element
             for (int i0 = (int)rank; i0 < L; i0 += (int)C * (NT / 16)) {
                 const int i = i0 + (int)C * (tid / 16);
@@ -548,7 +572,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
             cluster.sync();                  // pick is there, and no list is read any more
             const uint32_t tau = sm.pick;
             above = sm.pick_above;
-            if (MASS && level == 1) {
+            if (MASS && level == 1 && !few) {
                 // this slice above tau: its bins before the threshold's, and what the list adds
                 long long mass = 0;
                 for (int b = tid; b < pick; b += NT) mass += (long long)(((unsigned long long)sm.hi[b] << 32) | sm.lo[b]);
@@ -578,7 +602,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
         lo_key = kl_list;
         hi_key = kh;
         shift = 0;
-        while ((hi_key - kl) >> shift >= FBINS) shift++;
+        while ((hi_key - (with_floor ? floor_key : lo_key)) >> shift >= FBINS) shift++;
         cluster.sync();                      // before the histogram and the list are written again
     }
 }
@@ -664,11 +688,11 @@ __global__ void __launch_bounds__(NT, FS_OCC(NT)) k_sample_filtered(const float 
         } else {
             if (k < n) {
                 goal = k;
-                tau = select<NT, RESIDENT, false>(R, sm, 0, 0, 0.0, goal, above, own, own_ties);
+                tau = select<NT, RESIDENT, false>(R, sm, 0, 0, false, 0.0, goal, above, own, own_ties);
                 ties = k - above;
             }
             if (p < 1.f) {
-                tau = select<NT, RESIDENT, true>(R, sm, tau, ties, (double)p, goal, above, own, own_ties);
+                tau = select<NT, RESIDENT, true>(R, sm, tau, ties, k <= CAP, (double)p, goal, above, own, own_ties);
                 const long long w = R.units(key_value(tau));
                 ties = (goal - above + w - 1) / w;
             }
