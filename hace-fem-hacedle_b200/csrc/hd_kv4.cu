@@ -138,6 +138,7 @@ int hd_kv4_check(hd_ctx *ctx, const char *name, const void *cache, int64_t pages
                "%s: head_dim %d (32, 64 or 128)", name, head_dim);
     HD_REQUIRE(ctx, pages < ((int64_t)1 << 31) / page_size, HD_E_SHAPE, "%s: %lld pages of %d: 2^31 slots or more", name,
                (long long)pages, page_size);
+    HD_REQUIRE(ctx, (int64_t)n_kv * head_dim < ((int64_t)1 << 31), HD_E_SHAPE, "%s: %d kv heads of %d", name, n_kv, head_dim);
     HD_REQUIRE(ctx, ((uintptr_t)cache & 15) == 0, HD_E_ARG, "%s: the cache must be 16-byte aligned", name);
     return HD_OK;
 }

@@ -17,7 +17,7 @@ int hd_kv4_attention_check(hd_ctx *ctx, const char *name, Kv4Args &A, int page_s
     if (rc) return rc;
     HD_REQUIRE(ctx, A.n_heads > 0 && A.n_heads % A.n_kv == 0 && A.n_heads / A.n_kv <= MAXREP4, HD_E_SHAPE,
                "%s: n_heads %d must be a multiple of n_kv %d, at most %d per kv head", name, A.n_heads, A.n_kv, MAXREP4);
-    HD_REQUIRE(ctx, A.seqs >= 0 && A.rows >= 0 && A.rows < ((int64_t)1 << 31) && A.max_pages > 0 &&
+    HD_REQUIRE(ctx, A.seqs >= 0 && A.seqs < 1 << 30 && A.rows >= 0 && A.rows < ((int64_t)1 << 31) && A.max_pages > 0 &&
                         (int64_t)A.max_pages * page_size < ((int64_t)1 << 31),
                HD_E_SHAPE, "%s: bad shape (requests %d, rows %lld, table width %d)", name, A.seqs, (long long)A.rows,
                A.max_pages);

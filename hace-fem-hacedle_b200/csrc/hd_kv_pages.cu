@@ -76,7 +76,7 @@ __device__ __forceinline__ int find_run(const int *s, int n, int v) {
 __global__ void __launch_bounds__(PNT) k_pages_assign(const int32_t *lens, const int32_t *__restrict__ nnew, int reqs,
                                                       int32_t *tables, int max_pages, int shift,
                                                       const int32_t *__restrict__ free_list, const int32_t *n_free,
-                                                      int pages, int32_t *n_free_out, int32_t *lens_out,
+                                                      int free_cap, int pages, int32_t *n_free_out, int32_t *lens_out,
                                                       int32_t *__restrict__ row0, int32_t *__restrict__ slots,
                                                       int32_t *__restrict__ pos, int64_t max_rows,
                                                       int32_t *__restrict__ status) {
@@ -101,7 +101,10 @@ __global__ void __launch_bounds__(PNT) k_pages_assign(const int32_t *lens, const
     int64_t trows, tpages, arow = rows, apage = got;
     scan2(arow, apage, trows, tpages);
     bad = __syncthreads_or(bad);
-    const int st = bad ? PAGES_BAD_REQUEST : tpages > have_free ? PAGES_SHORT : trows > max_rows ? PAGES_ROWS : PAGES_OK;
+    const int st = bad || have_free < 0 || have_free > free_cap ? PAGES_BAD_REQUEST
+                   : tpages > have_free                         ? PAGES_SHORT
+                   : trows > max_rows                           ? PAGES_ROWS
+                                                                : PAGES_OK;
     for (int r = b; r < e; r++) {
         const int l = lens[r], n = st == PAGES_OK ? nnew[r] : 0;
         r0[r] = st == PAGES_OK ? (int)arow : 0;
@@ -177,7 +180,7 @@ __global__ void __launch_bounds__(PNT) k_pages_release(const int32_t *__restrict
     int64_t at = got;
     scan2(at, none, tp, tn);
     bad = __syncthreads_or(bad);
-    const int st = bad || have < 0 ? PAGES_BAD_REQUEST : have + tp > free_cap ? PAGES_SHORT : PAGES_OK;
+    const int st = bad || have < 0 || have > free_cap ? PAGES_BAD_REQUEST : have + tp > free_cap ? PAGES_SHORT : PAGES_OK;
     if (tid == 0) *status = st;
     if (st != PAGES_OK) return;
     for (int r = b; r < e; r++) {
@@ -219,17 +222,17 @@ int check_pages(hd_ctx *ctx, const char *name, int reqs, int max_pages, int page
 
 extern "C" int hd_kv_pages_assign(hd_ctx *ctx, const int32_t *lens, const int32_t *new_tokens, int reqs, int32_t *tables,
                                   int max_pages, int page_size, int pages, const int32_t *free_list,
-                                  const int32_t *n_free, int32_t *n_free_out, int32_t *lens_out, int32_t *row0,
+                                  const int32_t *n_free, int free_cap, int32_t *n_free_out, int32_t *lens_out, int32_t *row0,
                                   int32_t *slots, int32_t *pos, int64_t max_rows, int32_t *status) {
     if (!n_free || !n_free_out || !row0 || !status || (reqs > 0 && (!lens || !new_tokens || !tables || !lens_out)) ||
-        (max_rows > 0 && (!slots || !pos)) || (pages > 0 && !free_list))
+        (max_rows > 0 && (!slots || !pos)) || (free_cap > 0 && !free_list))
         return hd_fail(ctx, HD_E_ARG, "hd_kv_pages_assign: null argument");
     int rc = check_pages(ctx, "hd_kv_pages_assign", reqs, max_pages, page_size);
     if (rc) return rc;
-    HD_REQUIRE(ctx, max_rows >= 0 && max_rows < ((int64_t)1 << 31) && pages >= 0 &&
+    HD_REQUIRE(ctx, max_rows >= 0 && max_rows < ((int64_t)1 << 31) && free_cap >= 0 && pages >= 0 &&
                         (int64_t)pages * page_size < ((int64_t)1 << 31),
-               HD_E_SHAPE, "hd_kv_pages_assign: bad shape (rows %lld, pages %d: fewer than 2^31 slots)",
-               (long long)max_rows, pages);
+               HD_E_SHAPE, "hd_kv_pages_assign: bad shape (rows %lld, free list of %d, pages %d: fewer than 2^31 slots)",
+               (long long)max_rows, free_cap, pages);
     if (!ctx) return HD_E_ARG;
     HdDevice on(ctx);
     const size_t smem = (size_t)(3 * reqs + 2) * sizeof(int);
@@ -239,7 +242,7 @@ extern "C" int hd_kv_pages_assign(hd_ctx *ctx, const int32_t *lens, const int32_
     const int64_t want = (max_rows + 4 * PNT - 1) / (4 * PNT);
     const int ctas = want < 1 ? 1 : want > 8 ? 8 : (int)want;
     HD_CUDA_TRY(ctx, hd_launch_cluster(ctx, k_pages_assign, dim3(ctas), dim3(PNT), smem, ctas, lens, new_tokens, reqs, tables,
-                                       max_pages, page_shift(page_size), free_list, n_free, pages, n_free_out, lens_out,
+                                       max_pages, page_shift(page_size), free_list, n_free, free_cap, pages, n_free_out, lens_out,
                                        row0, slots, pos, max_rows, status));
     return HD_OK;
 }

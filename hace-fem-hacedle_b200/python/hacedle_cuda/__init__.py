@@ -109,7 +109,7 @@ def lib() -> C.CDLL:
         "hd_attention_decode_slots": [V, V, V, V, V, V, I, I, I, I, I, V],
         "hd_quantize_q8_1": [V, V, I, I64, V], "hd_qgemv_q8_1": [V, V, V, V, I],
         "hd_sample_filtered": [V, V, I64, I64, I64, V, V, V, V, V, V],
-        "hd_kv_pages_assign": [V, V, V, I, V, I, I, I, V, V, V, V, V, V, V, I64, V],
+        "hd_kv_pages_assign": [V, V, V, I, V, I, I, I, V, V, I, V, V, V, V, V, I64, V],
         "hd_kv_pages_release": [V, V, V, I, V, I, I, V, V, I, V],
         "hd_kv4_cache_bytes": [I64, I, I, I], "hd_kv4_workspace_bytes": [V, I, I, I],
         "hd_kv4_append": [V, V, V, I64, I64, V, I64, I, I, V, I64, I],
@@ -312,7 +312,7 @@ class Context:
                 rows != pos.numel():
             raise ValueError(f"lens, new, lens_out, row0, slots or pos do not fit {reqs} requests")
         rc = lib().hd_kv_pages_assign(self.h, lens.data_ptr(), new.data_ptr(), reqs, tables.data_ptr(), width, page_size, pages,
-                                      free.data_ptr(), n_free.data_ptr(), n_free_out.data_ptr(), lens_out.data_ptr(),
+                                      free.data_ptr(), n_free.data_ptr(), free.numel(), n_free_out.data_ptr(), lens_out.data_ptr(),
                                       row0.data_ptr(), slots.data_ptr(), pos.data_ptr(), rows, status.data_ptr())
         if rc:
             self._check(rc)

@@ -447,19 +447,22 @@ int hd_attention_decode_slots(hd_ctx *ctx, const float *q_dev, const float *kc_d
  *   lens_out_dev [reqs], n_free_out_dev [1]  the state after the step; they may
  *                         be lens_dev and n_free_dev themselves
  *   status_dev [1]        0; 1: the free pages do not suffice; 2: a length or
- *                         count is negative or beyond max_pages * page_size;
- *                         3: more than max_rows rows.  With 1..3 nothing is
+ *                         count is negative or beyond max_pages * page_size, or
+ *                         the free count is not in [0, free_cap]; 3: more than
+ *                         max_rows rows.  With 1..3 nothing is
  *                         placed: tables, lengths and the free count stay, row0
  *                         is all 0 and every slot -1.
- * Up to 8192 requests.  free_dev must hold *n_free_dev ids. */
+ * Up to 8192 requests.  free_dev holds free_cap ids, of which the first
+ * *n_free_dev are free. */
 int hd_kv_pages_assign(hd_ctx *ctx, const int32_t *lens_dev, const int32_t *new_dev, int reqs, int32_t *tables_dev,
                        int max_pages, int page_size, int pages, const int32_t *free_dev, const int32_t *n_free_dev,
-                       int32_t *n_free_out_dev, int32_t *lens_out_dev, int32_t *row0_dev, int32_t *slots_dev,
+                       int free_cap, int32_t *n_free_out_dev, int32_t *lens_out_dev, int32_t *row0_dev, int32_t *slots_dev,
                        int32_t *pos_dev, int64_t max_rows, int32_t *status_dev);
 /* Returns the pages of every request with done_dev[r] != 0 to the end of the
  * free stack (request order, table order), sets its length to 0 and its table
  * entries to -1.  free_cap: ids free_dev has room for.  status_dev: 0; 1: they
- * would not fit; 2: a length is out of range; with 1 and 2 nothing changes. */
+ * would not fit; 2: a length or the free count is out of range; with 1 and 2
+ * nothing changes. */
 int hd_kv_pages_release(hd_ctx *ctx, const int32_t *done_dev, int32_t *lens_dev, int reqs, int32_t *tables_dev,
                         int max_pages, int page_size, int32_t *free_dev, int32_t *n_free_dev, int free_cap,
                         int32_t *status_dev);
@@ -498,13 +501,16 @@ int hd_kv4_read(hd_ctx *ctx, const uint8_t *cache_dev, int64_t pages, int page_s
  * q_ld floats (0: dense; 16-byte aligned); out dense.  f32 accuracy: the
  * cache's values enter exactly, q and the softmax weights in two f16 parts.
  * decode:  row r is request r's last position, lens_dev[r] - 1.
- *          ws_dev: hd_kv4_workspace_bytes bytes, zeroed once before their first
- *          use, for calls that share nothing else in flight; NULL: the
- *          context's own (two graphs that may replay at the same time need one
- *          workspace each).
+ *          ws_dev: hd_kv4_workspace_bytes bytes (16-byte aligned), zeroed once
+ *          before their first use; calls that may run at the same time (two
+ *          streams, two graphs) need one each.  NULL: the context's own, made by
+ *          its first such call, which must not be captured.
  * prefill: rows row0[r] .. row0[r+1]-1 are the last positions of request r
- *          (row0_dev [seqs + 1] ascending from 0); rows: of q and out; those
- *          from row0[seqs] on are left as they are. */
+ *          (row0_dev [seqs + 1] ascending from 0, row0[seqs] <= rows); rows: of
+ *          q and out; those from row0[seqs] on are left as they are.  A request's
+ *          positions are walked by one CTA per 128 query rows and kv head, so a
+ *          single token behind a very long cache is better decoded.  A wait of
+ *          the kernel that runs out is reported by hd_ctx_check_device_errors. */
 uint64_t hd_kv4_workspace_bytes(const hd_ctx *ctx, int n_heads, int n_kv, int head_dim);
 int hd_kv4_attention_decode(hd_ctx *ctx, const float *q_dev, int64_t q_ld, const uint8_t *cache_dev, int64_t pages,
                             int page_size, const int32_t *tables_dev, int max_pages, const int32_t *lens_dev, int seqs,

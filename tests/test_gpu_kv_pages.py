@@ -57,7 +57,8 @@ def test_assign_matches_the_plain_loop(ctx, reqs, page, max_len, max_new, extra,
     assert len(set(slots)) == len(slots)          # no slot twice
 
 
-@pytest.mark.parametrize("what,status", [("short", 1), ("negative_len", 2), ("negative_new", 2), ("too_long", 2), ("rows", 3)])
+@pytest.mark.parametrize("what,status", [("short", 1), ("negative_len", 2), ("negative_new", 2), ("too_long", 2), ("rows", 3),
+                                         ("free_count", 2)])
 def test_a_step_that_does_not_fit_changes_nothing(ctx, what, status):
     import torch
     rng = np.random.default_rng(5)
@@ -70,6 +71,8 @@ def test_a_step_that_does_not_fit_changes_nothing(ctx, what, status):
         lens[1] = -1
     elif what == "negative_new":
         new[2] = -5
+    elif what == "free_count":
+        n_free = len(free) + 1               # more than the list holds
     elif what == "too_long":
         new[3] = 2 ** 31 - 1
     else:

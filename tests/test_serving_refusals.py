@@ -11,11 +11,11 @@ P = 4096       # a non-null, 16-byte aligned address that is never read
 OK = None
 
 
-def assign(reqs=4, width=8, page=16, pages=32, rows=64, **null):
+def assign(reqs=4, width=8, page=16, pages=32, rows=64, cap=32, **null):
     a = {n: P for n in ("lens", "new", "tables", "free", "n_free", "n_free_out", "lens_out", "row0", "slots", "pos", "status")}
     a.update({n: None for n in null})
     return hc.lib().hd_kv_pages_assign(None, a["lens"], a["new"], reqs, a["tables"], width, page, pages, a["free"],
-                                       a["n_free"], a["n_free_out"], a["lens_out"], a["row0"], a["slots"], a["pos"], rows,
+                                       a["n_free"], cap, a["n_free_out"], a["lens_out"], a["row0"], a["slots"], a["pos"], rows,
                                        a["status"])
 
 
@@ -57,10 +57,11 @@ def test_a_good_call_without_a_context_is_refused(call):
     (assign, {"slots": 1}, hc.HD_E_ARG), (assign, {"reqs": -1}, hc.HD_E_SHAPE), (assign, {"width": 0}, hc.HD_E_SHAPE),
     (assign, {"page": 8}, hc.HD_E_SHAPE), (assign, {"page": 48}, hc.HD_E_SHAPE), (assign, {"page": 2048}, hc.HD_E_SHAPE),
     (assign, {"reqs": 8193}, hc.HD_E_UNSUPPORTED), (assign, {"width": 1 << 27}, hc.HD_E_SHAPE),
-    (assign, {"rows": -1}, hc.HD_E_SHAPE), (assign, {"rows": 1 << 31}, hc.HD_E_SHAPE), (assign, {"pages": 1 << 27}, hc.HD_E_SHAPE),
+    (assign, {"rows": -1}, hc.HD_E_SHAPE), (assign, {"cap": -1}, hc.HD_E_SHAPE), (assign, {"rows": 1 << 31}, hc.HD_E_SHAPE),
+    (assign, {"pages": 1 << 27}, hc.HD_E_SHAPE),
     (release, {"page": 24}, hc.HD_E_SHAPE), (release, {"cap": -1}, hc.HD_E_SHAPE), (release, {"status": None}, hc.HD_E_ARG),
     (append, {"k": None}, hc.HD_E_ARG), (append, {"cache": None}, hc.HD_E_ARG), (append, {"hd": 80}, hc.HD_E_UNSUPPORTED),
-    (append, {"n_kv": 0}, hc.HD_E_SHAPE), (append, {"page": 0}, hc.HD_E_SHAPE), (append, {"pages": 1 << 27}, hc.HD_E_SHAPE),
+    (append, {"n_kv": 0}, hc.HD_E_SHAPE), (append, {"n_kv": 1 << 26, "rows": 1}, hc.HD_E_SHAPE), (append, {"page": 0}, hc.HD_E_SHAPE), (append, {"pages": 1 << 27}, hc.HD_E_SHAPE),
     (append, {"kld": 64}, hc.HD_E_SHAPE), (append, {"vld": 129}, hc.HD_E_ARG), (append, {"k": P + 4}, hc.HD_E_ARG),
     (append, {"cache": P + 8}, hc.HD_E_ARG), (append, {"rows": -1}, hc.HD_E_SHAPE), (append, {"rows": 1 << 33}, hc.HD_E_SHAPE),
     (read, {"slots": None}, hc.HD_E_ARG), (read, {"v": P + 4}, hc.HD_E_ARG), (read, {"hd": 96}, hc.HD_E_UNSUPPORTED),
@@ -69,7 +70,7 @@ def test_a_good_call_without_a_context_is_refused(call):
     (decode, {"sinks": -1}, hc.HD_E_ARG), (decode, {"scale": -1.0}, hc.HD_E_ARG), (decode, {"scale": float("nan")}, hc.HD_E_ARG),
     (decode, {"scale": float("inf")}, hc.HD_E_ARG), (decode, {"q": P + 4}, hc.HD_E_ARG), (decode, {"ld": 128}, hc.HD_E_SHAPE),
     (decode, {"ld": 258}, hc.HD_E_ARG), (decode, {"width": 0}, hc.HD_E_SHAPE), (decode, {"lens": None}, hc.HD_E_ARG),
-    (decode, {"seqs": -1}, hc.HD_E_SHAPE), (decode, {"hd": 256}, hc.HD_E_UNSUPPORTED), (decode, {"cache": P + 8}, hc.HD_E_ARG),
+    (decode, {"seqs": -1}, hc.HD_E_SHAPE), (prefill, {"seqs": 1 << 30}, hc.HD_E_SHAPE), (decode, {"hd": 256}, hc.HD_E_UNSUPPORTED), (decode, {"cache": P + 8}, hc.HD_E_ARG),
     (prefill, {"row0": None}, hc.HD_E_ARG), (prefill, {"rows": -1}, hc.HD_E_SHAPE), (prefill, {"rows": 1 << 31}, hc.HD_E_SHAPE),
     (prefill, {"out": None}, hc.HD_E_ARG), (prefill, {"page": 20}, hc.HD_E_SHAPE),
     (sample, {"u": None}, hc.HD_E_ARG), (sample, {"idx": None}, hc.HD_E_ARG), (sample, {"n": 0}, hc.HD_E_SHAPE),
