@@ -33,10 +33,7 @@
 
 namespace {
 
-#ifndef KV4_DW
-#define KV4_DW 4
-#endif
-constexpr int DW = KV4_DW;      // warps per CTA
+constexpr int DW = 4;           // warps per CTA
 constexpr int DNT = 32 * DW;
 constexpr int DPT = 2;          // tiles per step
 template <int HD>
@@ -47,11 +44,7 @@ constexpr int DCOST = 16;       // what beginning an item costs, in tiles
 constexpr int DJOIN = 16;       // CTAs whose partials are joined first
 constexpr int DJOINS = 64;      // partials that one CTA joins at a time, at most
 
-#ifndef KV4_WARPS
-#define KV4_WARPS 16
-#endif
-template <int HD>
-constexpr int d_occ() { return KV4_WARPS / DW; }   // CTAs per SM
+constexpr int D_OCC = 4;        // CTAs per SM (128 registers a thread)
 
 template <int HD>
 struct DShared {
@@ -187,7 +180,7 @@ __device__ void join_parts(DShared<HD> &sm, float *parts, float2 *ml, int n, Slo
 __device__ __forceinline__ int cost_of(const Seen &s) { return s.units ? s.units + DCOST : 0; }
 
 template <int HD>
-__global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int groups, int gh, int *tickets, float2 *ml,
+__global__ void __launch_bounds__(DNT, D_OCC) k_kv4_decode(Kv4Args A, int groups, int gh, int *tickets, float2 *ml,
                                                                float *parts) {
     constexpr int NS = d_stages<HD>();
     constexpr int WPT = HD / 32;       // words of a key per thread
@@ -552,8 +545,9 @@ __global__ void __launch_bounds__(DNT, d_occ<HD>()) k_kv4_decode(Kv4Args A, int 
     }
 }
 
-// CTAs of the largest grid.
-int max_ctas(const hd_ctx *ctx, int hd) { return min(ctx->sm_count * (hd == 128 ? d_occ<128>() : d_occ<64>()), DJOIN * DJOINS); }
+// CTAs of the largest grid, the same for every head size: the workspace's tickets are then, too, and one
+// workspace serves calls of several.
+int max_ctas(const hd_ctx *ctx) { return min(ctx->sm_count * D_OCC, DJOIN * DJOINS); }
 
 template <int HD>
 cudaError_t launch(hd_ctx *ctx, const Kv4Args &A, uint8_t *ws) {
@@ -569,7 +563,7 @@ cudaError_t launch(hd_ctx *ctx, const Kv4Args &A, uint8_t *ws) {
         tiles = tiles < seen ? tiles : seen;
     }
     const int64_t tiles_items = (int64_t)A.seqs * A.n_kv * groups, units = tiles * tiles_items;
-    const int64_t most = max_ctas(ctx, HD);
+    const int64_t most = max_ctas(ctx);
     const int64_t want = (units + tiles_items * DCOST + DMIN - 1) / DMIN;
     const int grid = (int)(want < most ? want : most);
     float2 *ml = (float2 *)(ws + ((size_t)3 * most * sizeof(int) + 255) / 256 * 256);
@@ -581,7 +575,7 @@ cudaError_t launch(hd_ctx *ctx, const Kv4Args &A, uint8_t *ws) {
 
 extern "C" uint64_t hd_kv4_workspace_bytes(const hd_ctx *ctx, int n_heads, int n_kv, int head_dim) {
     if (!ctx || n_heads <= 0 || n_kv <= 0 || (head_dim != 32 && head_dim != 64 && head_dim != 128)) return 0;
-    const uint64_t g = (uint64_t)max_ctas(ctx, head_dim);
+    const uint64_t g = (uint64_t)max_ctas(ctx);
     return (3 * g * sizeof(int) + 255) / 256 * 256 + 2 * g * DHEADS * (head_dim + 2) * sizeof(float);
 }
 
@@ -604,7 +598,7 @@ extern "C" int hd_kv4_attention_decode(hd_ctx *ctx, const float *q, int64_t q_ld
             HD_REQUIRE(ctx, capturing == cudaStreamCaptureStatusNone, HD_E_CUDA,
                        "hd_kv4_attention_decode: the context's workspace is made by the first call, which must not be "
                        "captured (or pass a workspace)");
-            const size_t most = (size_t)hd_kv4_workspace_bytes(ctx, 1, 1, 128) + (size_t)hd_kv4_workspace_bytes(ctx, 1, 1, 64);
+            const size_t most = (size_t)hd_kv4_workspace_bytes(ctx, 1, 1, 128);
             void *p = nullptr;
             if (cudaMalloc(&p, most) != cudaSuccess) {
                 cudaGetLastError();
@@ -616,8 +610,7 @@ extern "C" int hd_kv4_attention_decode(hd_ctx *ctx, const float *q, int64_t q_ld
             }
             ctx->kv4_ws = (uint8_t *)p;
         }
-        // the tickets of another head size's layout would meet this one's partials
-        ws = ctx->kv4_ws + (head_dim == 128 ? 0 : (size_t)hd_kv4_workspace_bytes(ctx, 1, 1, 128));
+        ws = ctx->kv4_ws;
     }
     cudaError_t e;
     if (head_dim == 128) e = launch<128>(ctx, A, (uint8_t *)ws);

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             mbar_init(smem_u32(&sm.v_full[s]), P_DEQ);
             mbar_init(smem_u32(&sm.s_full[s]), 2);         // the MMAs, and their issuer
             mbar_init(smem_u32(&sm.p_full[s]), P_SOFT);
-            mbar_init(smem_u32(&sm.pv_done[s]), 1);
+            mbar_init(smem_u32(&sm.pv_done[s]), 2);        // likewise
             mbar_init(smem_u32(&sm.fin[s]), 1);
         }
         mbar_init(smem_u32(&sm.raw_full), 1);
@@ -558,6 +558,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                     mma_ts(d, a + 16, bd, id_o, 1);
                 }
                 commit(smem_u32(&sm.pv_done[s]));
+                mbar_arrive(smem_u32(&sm.pv_done[s]));         // (hands on the bit masks of the unpacking warps)
             }
         }
         // what was issued ends before tensor memory is freed, also after a wait that ran out

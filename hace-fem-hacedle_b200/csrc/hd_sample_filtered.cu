@@ -41,11 +41,6 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-#ifndef FS_NT
-#define FS_NT 512
-#define FS_HALF 19456
-#define FS_OCC(NT) (1024 / NT)
-#endif
 constexpr int FBINS = 1024, FGROUP = 16, FGROUPS = FBINS / FGROUP;   // FGROUPS: also the first histogram's bins
 constexpr int CANDS = 2048;                  // elements of the first histogram's bin that a slice lists
 constexpr int CAP = 512;                     // elements compared with one another
@@ -608,7 +603,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
 }
 
 template <int NT, bool RESIDENT>
-__global__ void __launch_bounds__(NT, FS_OCC(NT)) k_sample_filtered(const float *__restrict__ logits, int64_t ld, int64_t n,
+__global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *__restrict__ logits, int64_t ld, int64_t n,
                                                                    const float *__restrict__ temp,
                                                                    const int32_t *__restrict__ top_k,
                                                                    const float *__restrict__ top_p,
@@ -823,7 +818,7 @@ extern "C" int hd_sample_filtered(hd_ctx *ctx, const float *logits, int64_t ld, 
     HdDevice on(ctx);
     // CTAs per row: as few as keep a slice at 80 KB, so that two CTAs share an SM; more while the rows
     // alone leave SMs idle and a slice keeps 2048 elements
-    constexpr int64_t HALF = FS_HALF;
+    constexpr int64_t HALF = 19456;
     auto slice_of = [&](int c) { return ((n + c - 1) / c + 3) / 4 * 4; };
     int C = 1;
     while (C < MAXC && (slice_of(C) > HALF || (rows * C < ctx->sm_count && slice_of(C) > 4096))) C *= 2;
@@ -841,7 +836,7 @@ extern "C" int hd_sample_filtered(hd_ctx *ctx, const float *logits, int64_t ld, 
     const double unit = std::ldexp(1.0, bits);
     const bool few = rows * C <= ctx->sm_count;   // one CTA an SM: twice the threads
 #define HD_SAMPLE(NT, RES) launch<NT, RES>(ctx, C, rows, slice, logits, ld, n, temperature, top_k, top_p, min_p, u, unit, half, idx)
-    cudaError_t e = slice > FULL ? HD_SAMPLE(1024, false) : few ? HD_SAMPLE(1024, true) : HD_SAMPLE(FS_NT, true);
+    cudaError_t e = slice > FULL ? HD_SAMPLE(1024, false) : few ? HD_SAMPLE(1024, true) : HD_SAMPLE(512, true);
 #undef HD_SAMPLE
     if (e != cudaSuccess) return hd_fail(ctx, HD_E_CUDA, "hd_sample_filtered: %s", cudaGetErrorString(e));
     return HD_OK;

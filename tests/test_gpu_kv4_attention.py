@@ -221,6 +221,18 @@ def test_decode_is_repeatable_and_captured(ctx):
     assert e.value.code == hc.HD_E_SHAPE
 
 
+def test_decode_one_workspace_for_every_head_size(ctx):
+    """Calls of different head sizes after one another in the same bytes, the caller's and the context's."""
+    import torch
+    cases = [Case(12 + hd, [2500, 3, 900], 1, hd, 32).device(torch) for hd in (32, 64, 128)]
+    ws = torch.zeros(max(ctx.kv4_workspace_bytes(8, 1, hd) for hd in (32, 64, 128)), dtype=torch.uint8, device="cuda")
+    qs = [c.rng.standard_normal((3, 8, c.hd)).astype(np.float32) for c in cases]
+    want = [_decode(ctx, torch, c, 8, q=q, ws=torch.zeros_like(ws))[1] for c, q in zip(cases, qs)]
+    for i in (0, 1, 2, 1, 0, 2, 0):
+        for w in (ws, None):
+            assert torch.equal(_decode(ctx, torch, cases[i], 8, q=qs[i], ws=w)[1], want[i])
+
+
 def _prefill(ctx, torch, c, heads, new, window=0, sinks=0, pad=0, q=None):
     row0 = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
     q = c.rng.standard_normal((row0[-1] + pad, heads, c.hd)).astype(np.float32) if q is None else q

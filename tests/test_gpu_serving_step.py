@@ -74,3 +74,58 @@ def test_serving_steps(ctx, page, window, sinks):
     assert checked > 100 and drawn >= 14 * reqs - 2
     held = sum(-(-len(m[0]) // page) for m in model)
     assert n_free.item() == pages - held
+
+
+def test_a_captured_step_follows_the_state(ctx):
+    """One graph holds a whole step; replayed, it does what the calls do one by one, also once the pages run out."""
+    import torch
+    rng = np.random.default_rng(77)
+    reqs, heads, n_kv, hd, page, pages, width, steps = 4, 8, 2, 64, 16, 9, 4, 24
+    up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    free = up(rng.permutation(pages).astype(np.int32))
+    one = torch.ones(reqs, dtype=torch.int32, device="cuda")
+
+    def state():
+        return {"cache": torch.zeros(hc.kv4_cache_shape(pages, page, n_kv, hd), dtype=torch.uint8, device="cuda"),
+                "tables": i32(reqs, width) - 1, "n_free": i32(1) + pages, "lens": i32(reqs),
+                "row0": i32(reqs + 1), "slots": i32(6), "pos": i32(6), "st": i32(1), "idx": i32(reqs),
+                "out": torch.zeros(reqs, heads, hd, device="cuda")}
+
+    qkv, u = torch.zeros(6, (heads + 2 * n_kv) * hd, device="cuda"), torch.zeros(reqs, device="cuda")
+    ws = [torch.zeros(ctx.kv4_workspace_bytes(heads, n_kv, hd), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    top_p = torch.full((reqs,), 0.8, device="cuda")
+
+    def step(s, w):
+        k = qkv[:, heads * hd:(heads + n_kv) * hd].unflatten(1, (n_kv, hd))
+        v = qkv[:, (heads + n_kv) * hd:].unflatten(1, (n_kv, hd))
+        ctx.kv_pages_assign(s["lens"], one, s["tables"], page, pages, free, s["n_free"], s["n_free"], s["lens"], s["row0"],
+                            s["slots"], s["pos"], s["st"])
+        ctx.kv4_append(k, v, s["slots"], s["cache"])
+        ctx.kv4_attention_decode(qkv[:reqs, :heads * hd].unflatten(1, (heads, hd)), s["cache"], s["tables"], s["lens"], s["out"],
+                                 window=20, sinks=2, ws=w)
+        ctx.sample_filtered(s["out"].view(reqs, -1), u, s["idx"], top_p=top_p)
+
+    eager, graphed = state(), state()
+    before, stream, g = torch.cuda.current_stream().cuda_stream, torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    step(state(), ws[0])                          # (shared memory limits are set outside the capture)
+    torch.cuda.synchronize()
+    ctx.set_stream(stream.cuda_stream)
+    try:
+        with torch.cuda.graph(g, stream=stream):
+            step(graphed, ws[1])
+    finally:
+        ctx.set_stream(before)
+    codes = []
+    for _ in range(steps * 2):
+        qkv.copy_(torch.from_numpy(rng.standard_normal(tuple(qkv.shape)).astype(np.float32)))
+        u.copy_(torch.from_numpy(rng.random(reqs).astype(np.float32)))
+        step(eager, ws[0])
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for n in eager:
+            assert torch.equal(eager[n], graphed[n]), n
+        codes.append(eager["st"].item())
+    # 9 pages hold two for each of four requests and one more: the 33rd token does not fit
+    assert codes == [0] * 32 + [1] * (steps * 2 - 32)
