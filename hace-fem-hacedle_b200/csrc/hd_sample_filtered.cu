@@ -20,9 +20,20 @@
 // many equal logits -- are split again).  Min-p is a smallest key, found by search.  The draw adds
 // up contiguous parts per CTA and per warp and follows the target down.
 //
-// The first histogram has a copy per lane, a bank each: atomics on shared
-// memory were what bounded a single one (13 of 33 us per row, against 4 for
-// the weights), since logits crowd into few bins.
+// The first histogram has a copy per lane, a bank each: with a single one the
+// atomics on shared memory were 13 of a row's 33 us, since logits crowd into
+// few bins.  A place in the list is found for 16 elements of a thread at a
+// time (4: 1.5 us more per row), and the search for a bin's bounds tries the
+// keys next to the computed one first (1.2 us less).
+//
+// 256 rows of 151936 logits with top-p 0.95 take 0.32 ms (156 MB: 24 us at the
+// measured copy rate), one row 31 us.  What bounds it: a row passes through
+// some 20 steps, eight of them behind a barrier of its cluster, of which only
+// the load, the first histogram (8 of 47 us per row, about 50 instructions an
+// element) and the list touch every element; registers allow two rows at a
+// time on an SM, so the steps in between leave it half idle (issue slots 46%
+// busy).  One CTA per row that reads its row from L2 again at every pass came
+// to the same time with top-k and to 0.5 ms with top-p.
 //
 // Weights are computed in 64 bits (2^y = 2^(j/256) 2^e 2^r with a table of 256
 // and a polynomial of degree 4 in r, |r| <= 1/512: the table-driven method of
@@ -135,7 +146,8 @@ struct FShared {
             uint32_t lane_lo[FGROUPS * 32], lane_hi[FGROUPS * 32];
         };
         struct {                             // the others, 64 bits in two halves; the listed elements
-            uint32_t lo[FBINS], hi[FBINS], cand[CANDS];
+            uint32_t lo[FBINS], hi[FBINS];
+            float cand[CANDS];
         };
     };
     long long part[MAXC][FGROUP];            // a group's bins of every CTA
@@ -187,72 +199,82 @@ template <int NT, bool RESIDENT, bool MASS>
 __device__ __noinline__ void first_histogram(FShared &sm, float least) {
     const Row R = sm.row;
     const int tid = threadIdx.x, lane = tid & 31;
-                const uint32_t low = (1u << R.half) - 1;
-                auto count = [&](float v, double y, double k, unsigned long long w) {
-                    const bool tiny = Row::tiny(y);
-                    const int at = Row::bin(tiny, k) * 32 + lane;
-                    if (!(v >= least)) return;
-                    if (!MASS) {
-                        atomicAdd(&sm.lane_lo[at], 1u);
-                    } else if (tiny) {
-                        return;
-                    } else if (RESIDENT) {       // neither half can overflow, and no atomic returns anything
-                        atomicAdd(&sm.lane_lo[at], (uint32_t)w & low);
-                        atomicAdd(&sm.lane_hi[at], (uint32_t)(w >> R.half));
-                    } else {
-                        add64(sm.lane_lo, sm.lane_hi, at, w);
-                    }
-                };
-                for (int i = tid; i < R.n4; i += NT) {
-                    const float4 v = R.four<RESIDENT>(i);
-                    if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least)) continue;
-                    double y[4], k[4];
-                    unsigned long long w[4] = {0, 0, 0, 0};
-                    y[0] = R.log2w(v.x, k[0]);
-                    y[1] = R.log2w(v.y, k[1]);
-                    y[2] = R.log2w(v.z, k[2]);
-                    y[3] = R.log2w(v.w, k[3]);
-                    if (MASS) {
-    #pragma unroll
-                        for (int c = 0; c < 4; c++) w[c] = (unsigned long long)Row::whole(R.weight(y[c], k[c]));
-                    }
-                    count(v.x, y[0], k[0], w[0]);
-                    count(v.y, y[1], k[1], w[1]);
-                    count(v.z, y[2], k[2], w[2]);
-                    count(v.w, y[3], k[3], w[3]);
-                }
+    const uint32_t low = (1u << R.half) - 1;
+    auto count = [&](float v, double y, double k, unsigned long long w) {
+        const bool tiny = Row::tiny(y);
+        const int at = Row::bin(tiny, k) * 32 + lane;
+        if (!(v >= least)) return;
+        if (!MASS) {
+            atomicAdd(&sm.lane_lo[at], 1u);
+        } else if (tiny) {
+            return;
+        } else if (RESIDENT) {       // neither half can overflow, and no atomic returns anything
+            atomicAdd(&sm.lane_lo[at], (uint32_t)w & low);
+            atomicAdd(&sm.lane_hi[at], __funnelshift_r((uint32_t)w, (uint32_t)(w >> 32), R.half));
+        } else {
+            add64(sm.lane_lo, sm.lane_hi, at, w);
+        }
+    };
+    for (int i = tid; i < R.n4; i += NT) {
+        const float4 v = R.four<RESIDENT>(i);
+        if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least)) continue;
+        double y[4], k[4];
+        unsigned long long w[4] = {0, 0, 0, 0};
+        y[0] = R.log2w(v.x, k[0]);
+        y[1] = R.log2w(v.y, k[1]);
+        y[2] = R.log2w(v.z, k[2]);
+        y[3] = R.log2w(v.w, k[3]);
+        if (MASS) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) w[c] = (unsigned long long)Row::whole(R.weight(y[c], k[c]));
+        }
+        count(v.x, y[0], k[0], w[0]);
+        count(v.y, y[1], k[1], w[1]);
+        count(v.z, y[2], k[2], w[2]);
+        count(v.w, y[3], k[3], w[3]);
+    }
 }
 
-// The keys of the elements lo .. hi into cand, in any order.
+// The elements lo .. hi into cand, in any order (once there are too many: only their number counts).
 template <int NT, bool RESIDENT>
 __device__ __noinline__ void list_bin(FShared &sm, float lo, float hi) {
+    constexpr int FOURS = 4;                 // a place for a thread's elements costs as much for 16 as for 4
     const Row R = sm.row;
     const int tid = threadIdx.x, lane = tid & 31;
-                            auto in = [&](float v) { return v >= lo && v <= hi; };
-                for (int i0 = 0; i0 < R.n4; i0 += NT) {
-                    const float4 v = i0 + tid < R.n4 ? R.four<RESIDENT>(i0 + tid) : make_float4(NAN, NAN, NAN, NAN);
-                    const int mine = (int)in(v.x) + in(v.y) + in(v.z) + in(v.w);
-                    if (!__any_sync(0xffffffffu, mine)) continue;
-                    int at = mine;               // a place for each lane's in the warp's run
-    #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const int x = __shfl_up_sync(0xffffffffu, at, o);
-                        if (lane >= o) at += x;
-                    }
-                    uint32_t base = 0;
-                    if (lane == 31) base = atomicAdd(&sm.n_cand, (uint32_t)at);
-                    uint32_t to = __shfl_sync(0xffffffffu, base, 31) + at - mine;
-                    auto put = [&](float x) {
-                        if (in(x)) {
-                            if (to < CANDS) sm.cand[to] = order_key(x);
-                            to++;
-                        }
-                    };
-                    put(v.x);
-                    put(v.y);
-                    put(v.z);
-                    put(v.w);
-                }
+    for (int i0 = 0; i0 < R.n4; i0 += FOURS * NT) {
+        float v[4 * FOURS];
+        bool in[4 * FOURS];
+        int mine = 0;
+#pragma unroll
+        for (int f = 0; f < FOURS; f++) {
+            const int i = i0 + f * NT + tid;
+            const float4 x = i < R.n4 ? R.four<RESIDENT>(i) : make_float4(NAN, NAN, NAN, NAN);
+            v[4 * f] = x.x;
+            v[4 * f + 1] = x.y;
+            v[4 * f + 2] = x.z;
+            v[4 * f + 3] = x.w;
+        }
+#pragma unroll
+        for (int c = 0; c < 4 * FOURS; c++) {
+            in[c] = v[c] >= lo && v[c] <= hi;
+            mine += in[c];
+        }
+        if (!__any_sync(0xffffffffu, mine)) continue;
+        int at = mine;                       // a place for each lane's in the warp's run
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += x;
+        }
+        uint32_t base = 0;
+        if (lane == 31 && at) base = atomicAdd(&sm.n_cand, (uint32_t)at);
+        base = __shfl_sync(0xffffffffu, base, 31);
+        float *to = sm.cand + base + at - mine;
+        if (!mine || base + at > CANDS) continue;
+#pragma unroll
+        for (int c = 0; c < 4 * FOURS; c++)
+            if (in[c]) *to++ = v[c];
+    }
 }
 
 // A warp's fours b .. e - 1: their weight above ft, and how many equal it.
@@ -292,11 +314,18 @@ __device__ __forceinline__ long long cluster_sum(unsigned C, F f) {
 }
 
 // The largest key <= top for which `low` holds, by a warp; it holds for
-// KEY_NINF, not for top, and for all keys below one for which it holds.
+// KEY_NINF, not for top, and for all keys below one for which it holds.  The
+// keys next to a guess are tried first.
 template <typename F>
-__device__ uint32_t last_key(uint32_t top, F low) {
+__device__ uint32_t last_key(uint32_t top, double guess, F low) {
     const int lane = threadIdx.x & 31;
     uint32_t lo = KEY_NINF, hi = top;
+    {
+        const int64_t c64 = (int64_t)order_key(plain((float)guess)) + lane - 16;
+        const uint32_t c = c64 < lo ? lo : c64 > hi ? hi : (uint32_t)c64;
+        const uint32_t high = ~__ballot_sync(0xffffffffu, c == lo || (c != hi && low(c)));
+        if (high & ~1u && !(high & 1u)) return __shfl_sync(0xffffffffu, c, __ffs(high) - 2);
+    }
     while (hi - lo > 1) {
         const uint32_t step = (hi - lo + 32) / 33;
         const uint64_t c64 = (uint64_t)lo + (uint64_t)step * (lane + 1);
@@ -316,12 +345,14 @@ __device__ uint32_t last_key(uint32_t top, F low) {
 // weight of the elements > tau.  Every CTA of the cluster gets the same.
 // `few`: the elements above the floor are at most CAP together (top-k has
 // left them): they are listed at once and compared, without a histogram.
+// `clear`: the first histogram is all zeros already.
 // `own` becomes the slice's own weight above tau and its elements equal to it
 // where the histogram tells (MASS, one level), and -1 elsewhere.
 template <int NT, bool RESIDENT, bool MASS>
-__device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long long floor_ties, bool few, double p,
+__device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long long floor_ties, bool few, bool clear, double p,
                            long long &goal, long long &above, long long &own, int &own_ties) {
     constexpr int NW = NT / 32;
+    static_assert(NW >= MAXC && NW <= MAXW, "a warp per CTA of the cluster");
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned C = cluster.num_blocks(), rank = cluster.block_rank();
@@ -337,7 +368,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
     // f(key) of each of them (and of the lanes' own pace; for few elements)
     auto each = [&](auto f) {
         if (listed) {
-            for (int i = tid; i < (int)sm.n_cand; i += NT) f(sm.cand[i]);
+            for (int i = tid; i < (int)sm.n_cand; i += NT) f(order_key(sm.cand[i]));
         } else {
             const float lo = key_value(lo_key), hi = key_value(hi_key);
             auto in = [&](float v) { if (v >= lo && v <= hi) f(order_key(v)); };
@@ -357,9 +388,10 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
             if (tid == 0) sm.n_list = 0;
             __syncthreads();
         } else {
-            if (level == 0)
-                for (int b = tid; b < FGROUPS * 32; b += NT) sm.lane_lo[b] = sm.lane_hi[b] = 0;
-            else
+            if (level == 0) {
+                if (!clear)
+                    for (int b = tid; b < FGROUPS * 32; b += NT) sm.lane_lo[b] = sm.lane_hi[b] = 0;
+            } else
                 for (int b = tid; b < FBINS; b += NT) sm.lo[b] = sm.hi[b] = 0;
             if (tid == 0) sm.n_list = 0;
             __syncthreads();
@@ -455,7 +487,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
             if (level == 0) {
                 if (warp < 2) {
                     const int v = pick + warp;   // the largest key of a bin >= v
-                    const uint32_t k = v == 0 ? order_key(R.top) : v >= FGROUPS ? KEY_NINF - 1 : last_key(order_key(R.top), [&](uint32_t c) { return R.bin(key_value(c)) >= v; });
+                    const uint32_t k = v == 0 ? order_key(R.top) : v >= FGROUPS ? KEY_NINF - 1 : last_key(order_key(R.top), R.m - (128.0 * v - 0.5) / 256 / R.a, [&](uint32_t c) { return R.bin(key_value(c)) >= v; });
                     if (lane == 0) sm.bound[warp] = k;
                 }
                 __syncthreads();
@@ -473,8 +505,7 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
                 return kl;
             }
             if (level == 0) {
-                if (MASS)
-                    for (int q = 0; q < pick; q++) own_above += sm.group[q];
+                if (MASS) own_above = warp_sum((lane < pick ? sm.group[lane] : 0) + (lane + 32 < pick ? sm.group[lane + 32] : 0));
                 lo_key = with_floor ? floor_key + 1 : kl;
                 hi_key = kh;
                 shift = 0;
@@ -584,11 +615,8 @@ __device__ uint32_t select(const Row &R, FShared &sm, uint32_t floor_key, long l
                     sm.wtie[warp] = tie;
                 }
                 __syncthreads();
-                own = own_above;
-                for (int w = 0; w < NW; w++) {
-                    own += sm.wsum[w];
-                    own_ties += sm.wtie[w];
-                }
+                own = own_above + warp_sum(lane < NW ? sm.wsum[lane] : 0);
+                own_ties = __reduce_add_sync(0xffffffffu, lane < NW ? sm.wtie[lane] : 0);
                 if (with_floor && tau == floor_key) own = -1;   // the floor's own are not in the list
                 __syncthreads();
             }
@@ -625,6 +653,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *
     R.n = (int)(end - begin);
     R.n4 = (R.n + 3) / 4;
     for (int i = tid; i < 256; i += NT) sm.table[i] = exp2((double)i / 256) * unit;
+    for (int b = tid; b < FGROUPS * 32; b += NT) sm.lane_lo[b] = sm.lane_hi[b] = 0;
     if (tid == 0) sm.kmax = 0;
     __syncthreads();
     pdl_wait();
@@ -683,17 +712,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *
         } else {
             if (k < n) {
                 goal = k;
-                tau = select<NT, RESIDENT, false>(R, sm, 0, 0, false, 0.0, goal, above, own, own_ties);
+                tau = select<NT, RESIDENT, false>(R, sm, 0, 0, false, true, 0.0, goal, above, own, own_ties);
                 ties = k - above;
             }
             if (p < 1.f) {
-                tau = select<NT, RESIDENT, true>(R, sm, tau, ties, k <= CAP, (double)p, goal, above, own, own_ties);
+                tau = select<NT, RESIDENT, true>(R, sm, tau, ties, k <= CAP, k == n, (double)p, goal, above, own, own_ties);
                 const long long w = R.units(key_value(tau));
                 ties = (goal - above + w - 1) / w;
             }
             if (mp > 0.0) {
                 // the smallest key with weight >= min_p
-                const uint32_t least = last_key(order_key(R.top), [&](uint32_t c) { return R.weight(key_value(c)) < mp * unit; }) + 1;
+                const uint32_t least = last_key(order_key(R.top), R.m + log2(mp) / R.a, [&](uint32_t c) { return R.weight(key_value(c)) < mp * unit; }) + 1;
                 if (least > tau) {
                     tau = least;
                     ties = n;
