@@ -13,24 +13,40 @@
 // (7e-6 of the result over 8192 positions, 4e-7 now), and the change of the
 // running maximum is one multiplication on the way.
 //
-// Roles (14 warps, one CTA per SM; S, P and PV have two buffers each in tensor
-// memory, K and V two stages in shared memory, so the four work on different
+// Roles (15 warps, one CTA per SM; S, P and PV have two buffers each in tensor
+// memory, K and V two stages in shared memory, so the roles work on different
 // tiles at a time):
 //   warps 0-7       softmax: a thread has a row and half of a tile's columns,
 //            and half of the row's dimensions of O; the two threads of a row
 //            exchange their maxima through shared memory.  P overwrites S in
-//            place: 32 scores become 16 + 16 columns of high and low parts.
-//   warps 8-11      fetch cache tiles by bulk copies and write K and V^T as
-//            f16 operands in SWIZZLE_128B.  K's dimensions keep the order in
-//            which nibbles unpack and Q is stored to match; V is paired by byte
-//            permutes, so neither is transposed through memory.
+//            place: CW scores become CW / 2 columns of high and CW / 2 of low
+//            parts.  Two f32 operations an instruction where they pair.
+//   warps 8-11      write K and V^T as f16 operands in SWIZZLE_128B from the
+//            cache tiles.  K's dimensions keep the order in which nibbles unpack
+//            and Q is stored to match; V is paired by byte permutes, so neither
+//            is transposed through memory.
 //   warp 12, 13     issue the MMAs of S and of PV: one thread for both was the
 //            pace (an MMA costs its issuer 60 to 80 cycles, 32 of them a tile).
+//   warp 14         fetches cache tiles by bulk copies, a position tile ahead
+//            (by one of the unpacking warps, the barrier among them and the page
+//            table's latency stood in each tile: 52 us against 46.6 below).
 //
 // A value that is not finite (a cache row quantized from a NaN) must reach the
 // rows that see its position and no other, but 0 * NaN is NaN: such values
 // enter V as 0 and are kept in a bit mask per position, which the rows that
 // see it take over for their output dimensions.
+//
+// Measured: 4096 rows on 8192 positions, 28 heads on 4 of 128 (361 GFLOP
+// counted once), 0.94 ms: 384 TFLOP/s, 769 of MMA work with the two parts of q
+// and P, 46% of the measured bf16 rate; chunks of 1 to 500 rows of 12 requests,
+// 14 heads on 2 of 64, 46.6 us.  What bounds it: the softmax warps and the
+// unpacking warps each take about 4.5 thousand cycles for 128 positions, the
+// MMAs 2.2 thousand.  No pipe is full (issue slots 52%, ALU 35%); after fixed
+// latencies the waits are for instructions, since either role runs through
+// its code once a tile.  Slower: 8 unpacking or 16 softmax warps (1.1 and 1.5
+// ms), registers moved from the issuing to the softmax warps (no spills, 1.1
+// ms), half of the scores kept in registers over the barrier (1.1 ms), the
+// unpacking loops rolled (1.03 ms).
 #include "hd_internal.cuh"
 #include "hd_kv4_math.cuh"
 #include "hd_tc.cuh"
@@ -39,9 +55,9 @@ namespace {
 
 constexpr int PM = 128, PN = 128;               // rows, positions per tile
 constexpr int P_SOFT = 256, P_DEQ = 128;        // threads of the softmax and of the unpacking warps
-constexpr int P_THREADS = P_SOFT + P_DEQ + 64;
+constexpr int P_THREADS = P_SOFT + P_DEQ + 96;
 constexpr int PG = PN / KV4_TILE;               // cache tiles per position tile
-constexpr int ABSENT = 0x40000000;              // position of a cache tile that is not there
+constexpr int ABSENT = 0x7ffffff0;              // position of a cache tile that is not there
 
 template <int HD>
 struct PLayout {
@@ -56,7 +72,7 @@ struct PLayout {
 };
 
 struct PShared {
-    unsigned long long k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], raw_full, fin[2];
+    unsigned long long k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], raw_full, raw_free, fin[2];
     uint32_t tmem;
     int pos[8][PG];               // first position of each cache tile of a position tile (read long after K is free)
     uint8_t nan_bits[4][4][PN / 8];   // which of 8 positions' values of a group are not finite
@@ -89,6 +105,20 @@ __device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&r)[32]) {
         "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(a)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t (&r)[32]) { tmem_ld32(a, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t (&r)[16]) {
+    tmem_ld16_async(a, r);
+    tmem_wait_ld();
+    tmem_regs_ready(r);
+}
+__device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t (&r)[32]) { tmem_st32(a, r); }
+__device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(a)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -102,12 +132,55 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+// Two f32 operations an instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// split2 of a pair.
+__device__ __forceinline__ void split_pair(uint64_t x, uint32_t &hi, uint32_t &lo) {
+    const float2 v = unpack2(x);
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    const float2 f = __half22float2(h), d = unpack2(fma2(pack2(f.x, f.y), pack2(-1.f, -1.f), x));
+    const __half2 l = __floats2half2_rn(d.x, d.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ bool not_finite(uint32_t d) { return (d & 0x7fffu) >= 0x7c00u; }
 
 template <int HD>
 __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq, int *flag) {
     using L = PLayout<HD>;
     constexpr int KS = HD / 16;                            // k-steps of the first product
+    // scores that a softmax thread takes at a time (16 for HD 64: 54 us for 12 short prompts, 46.5 with 32; 32 for HD
+    // 128: 1.06 ms for 4096 rows, 0.95 with 16: its two rolled loops then stay in the instruction cache)
+    constexpr int CW = HD == 128 ? 16 : 32;
     constexpr uint32_t S_COL = 0, PV_COL = 2 * PN;         // tensor memory: two buffers of S and P, then two of PV
     extern __shared__ uint8_t raw[];
     __shared__ PShared sm;
@@ -172,6 +245,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             mbar_init(smem_u32(&sm.fin[s]), 1);
         }
         mbar_init(smem_u32(&sm.raw_full), 1);
+        mbar_init(smem_u32(&sm.raw_free), P_DEQ / 32);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -225,9 +299,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const int i_row = i0 + r / rep, f_row = A.window && i_row >= A.window ? i_row - A.window + 1 : 0;
         constexpr int OD = HD / 2, OC = OD < 32 ? 16 : 32;     // this thread's dimensions, and how many it reads at once
-        float o[OD], m = -INFINITY, l = 0.f;
+        uint64_t o[OD / 2];                // pairs of dimensions
+        float m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int i = 0; i < OD; i++) o[i] = 0.f;
+        for (int i = 0; i < OD / 2; i++) o[i] = 0;
         uint32_t nan_mine = 0;
         bool alive = true;
         // the groups of tile j's values that are not finite, of positions that the row sees
@@ -249,18 +324,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             const uint32_t at = tmem + lanes + PV_COL + (j & 1) * HD + half * OD;
 #pragma unroll
             for (int c = 0; c < OD; c += OC) {
-                if constexpr (OC == 32) {
-                    uint32_t x[32];
-                    tmem_ld32(at + c, x);
+                {
+                    uint32_t x[OC];
+                    tmem_ld(at + c, x);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[c + i] += __uint_as_float(x[i]);
-                } else {
-                    uint32_t x[16];
-                    tmem_ld16_async(at + c, x);
-                    tmem_wait_ld();
-                    tmem_regs_ready(x);
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[c + i] += __uint_as_float(x[i]);
+                    for (int i = 0; i < OC / 2; i++)
+                        o[c / 2 + i] = add2(o[c / 2 + i], pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])));
                 }
             }
         };
@@ -273,14 +342,13 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             // s_full cannot run ahead, and its issuer's own arrival hands on what the unpacking warps wrote.
             alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.s_full[s]), k & 1, flag));
             tc_fence_after();
-            // scores of 32 columns, -infinity where the row does not see the position
-            auto load = [&](int c, float (&v)[32]) {
-                uint32_t (&u)[32] = reinterpret_cast<uint32_t (&)[32]>(v);
-                tmem_ld32(t_s + 32 * c, u);
+            // scores of CW columns, -infinity where the row does not see the position
+            auto load = [&](int c, float (&v)[CW]) {
+                tmem_ld(t_s + CW * c, reinterpret_cast<uint32_t (&)[CW]>(v));
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int p0 = sm.pos[j & 7][4 * half + 2 * c + h];
-                    const bool all = p0 + KV4_TILE - 1 <= i_row && (p0 >= f_row || p0 + KV4_TILE <= A.sinks);
+                for (int h = 0; h < CW / KV4_TILE; h++) {
+                    const int p0 = sm.pos[j & 7][PN / 2 / KV4_TILE * half + CW / KV4_TILE * c + h];
+                    const bool all = p0 + KV4_TILE - 1 <= i_row && (p0 >= f_row || p0 <= A.sinks - KV4_TILE);
                     if (__all_sync(0xffffffffu, all)) continue;
 #pragma unroll
                     for (int i = 0; i < KV4_TILE; i++) {
@@ -291,16 +359,16 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             };
             float mx = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < 2 && alive; c++) {
-                float v[32];
+            for (int c = 0; c < PN / 2 / CW && alive; c++) {
+                float v[CW];
                 load(c, v);
                 float a = v[0], b = v[1];
 #pragma unroll
-                for (int i = 2; i < 32; i += 2) {
-                    a = fmaxf(a, v[i]);
-                    b = fmaxf(b, v[i + 1]);
+                for (int i = 2; i < CW - 2; i += 4) {
+                    a = max3(a, v[i], v[i + 1]);
+                    b = max3(b, v[i + 2], v[i + 3]);
                 }
-                mx = fmaxf(mx, fmaxf(a, b));
+                mx = max3(mx, max3(a, b, v[CW - 2]), v[CW - 1]);
             }
             sm.mx[s][half][r] = mx;          // (the other buffer next time: one barrier a tile is enough)
             bar_sync(1, P_SOFT);
@@ -309,24 +377,23 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : exp2_approx(m - mn);
             m = mn;
             const float ref = m == -INFINITY ? 0.f : m - 15.f;
-            float sum = 0.f;
+            const uint64_t kappa2 = pack2(kappa, kappa), ref2 = pack2(-ref, -ref);
+            uint64_t sum = 0;
 #pragma unroll 1
-            for (int c = 0; c < 2; c++) {
-                float v[32];
+            for (int c = 0; c < PN / 2 / CW; c++) {
+                float v[CW];
                 load(c, v);
-                uint32_t p[32];
-                float l0 = 0.f, l1 = 0.f;
+                uint32_t p[CW];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float x = exp2_approx(fmaf(v[2 * i], kappa, -ref)), y = exp2_approx(fmaf(v[2 * i + 1], kappa, -ref));
-                    l0 += x;
-                    l1 += y;
-                    split2(x, y, p[i], p[16 + i]);
+                for (int i = 0; i < CW / 2; i++) {
+                    const float2 t = unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), kappa2, ref2));
+                    const uint64_t x = pack2(exp2_approx(t.x), exp2_approx(t.y));
+                    sum = add2(sum, x);
+                    split_pair(x, p[i], p[CW / 2 + i]);
                 }
-                sum += l0 + l1;
-                tmem_st32(t_s + 32 * c, p);
+                tmem_st(t_s + CW * c, p);
             }
-            l = fmaf(l, a, sum);
+            l = fmaf(l, a, unpack2(sum).x + unpack2(sum).y);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(smem_u32(&sm.p_full[s]));
@@ -334,7 +401,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             if (j > 0) take(j - 1);
             if (__any_sync(0xffffffffu, a != 1.f)) {
 #pragma unroll
-                for (int i = 0; i < OD; i++) o[i] *= a;
+                for (int i = 0; i < OD / 2; i++) o[i] = mul2(o[i], pack2(a, a));
             }
         }
         if (alive && nj > 0) take(nj - 1);
@@ -345,10 +412,11 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             float *out = A.out + (((int64_t)r_begin + t0 + r / rep) * A.n_heads + kvh * rep + r % rep) * HD + half * OD;
 #pragma unroll
             for (int i = 0; i < OD; i += 4) {
+                const float2 u = unpack2(o[i / 2]), w = unpack2(o[i / 2 + 1]);
                 const bool bad = nan_mine >> ((half * OD + i) / 32) & 1;
                 *(float4 *)(out + i) = i_row < 0 || total == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
                                        : bad ? make_float4(NAN, NAN, NAN, NAN)
-                                             : make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                                             : make_float4(u.x * inv, u.y * inv, w.x * inv, w.y * inv);
             }
         }
     } else if (warp < 12) {
@@ -363,50 +431,15 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
         const int v_piece = HD == 32 ? 0 : (vr >> 1) & (PIECES - 1);
         const int v_word = HD == 128 ? 2 * (vr >> 3) : HD == 64 ? vr >> 2 : (vr >> 1) & 3;
         const bool v_on = HD != 32 || vr < 8;
-        const int page_tiles = 1 << (A.shift - 4);
-        uint8_t *raw0 = base + 2 * L::Q + 2 * (L::K + L::V);
-        // lane i < 8: where cache tile i of position tile j lies, or -1; and its first position
-        auto look = [&](int j, int &pos) {
-            const int u = PG * j + (lane & 7);
-            pos = ABSENT;
-            if (u >= S.units) return -1;
-            const int tile = S.tile(u);
-            const int64_t page = table[tile >> (A.shift - 4)];
-            if (page < 0 || page >= A.pages) return -1;
-            pos = tile * KV4_TILE;
-            return (int)((page * A.n_kv + kvh) * page_tiles + (tile & (page_tiles - 1)));
-        };
-        // the copies of one position tile, by the first unpacking warp
-        auto copy = [&](int at) {
-            if (w4 != 0) return;
-            const int n = __popc(__ballot_sync(0xffffffffu, lane < PG && at >= 0));
-            const uint32_t bar = smem_u32(&sm.raw_full);
-            if (lane == 0)
-                asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n}\n" ::"r"(bar),
-                             "r"(n * kv4_tile_bytes(HD))
-                             : "memory");
-            __syncwarp();
-            if (lane < PG && at >= 0)
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                 smem_u32(raw0 + lane * L::RAW1)),
-                             "l"(A.cache + (uint64_t)(uint32_t)at * kv4_tile_bytes(HD)), "r"(kv4_tile_bytes(HD)), "r"(bar)
-                             : "memory");
-        };
-        int pos = ABSENT, pos_next = ABSENT;
+        const uint8_t *raw0 = base + 2 * L::Q + 2 * (L::K + L::V);
         bool alive = true;
-        int at = nj > 0 ? look(0, pos) : -1, in_flight = 0;
-        if (nj > 0) {
-            copy(at);
-            in_flight = 1;
-        }
-        int at_next = nj > 1 ? look(1, pos_next) : -1;
         for (int j = 0; j < nj; j++) {
             const int s = j & 1;
             alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.raw_full), j & 1, flag));
-            in_flight = alive ? 0 : in_flight;
+            if (!alive) break;
+            const int pos = sm.pos[j & 7][lane & (PG - 1)];
             // whether every position is seen by some row (else the scales of the others count as 0)
-            const bool whole = __all_sync(0xffffffffu, lane >= PG || (at >= 0 && pos + KV4_TILE - 1 <= S.last &&
-                                                                      (pos >= S.first || pos + KV4_TILE <= A.sinks)));
+            const bool whole = __all_sync(0xffffffffu, pos + KV4_TILE - 1 <= S.last && (pos >= S.first || pos <= A.sinks - KV4_TILE));
             uint4 kw[KI];
             uint32_t kd[KI], vw[8][VW], vd[8];
 #pragma unroll
@@ -443,20 +476,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
                 for (int i = 0; i < 8; i++)
                     if (!S.any(p0 + i, A.sinks)) vd[i] = 0;
             }
-            const int pos_here = pos;
-            bar_sync(2, P_DEQ);              // all four warps have read the raw tiles
-            if (j + 1 < nj && alive) {
-                at = at_next;
-                pos = pos_next;
-                copy(at);
-                in_flight = 1;
-                at_next = j + 2 < nj ? look(j + 2, pos_next) : -1;
-            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.raw_free));   // this warp has read the raw tiles
             // K's stage is free once the S that read it is there, V's once the PV is
             alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.s_full[s]), ((j >> 1) & 1) ^ 1, flag));
-            if (!alive) continue;              // (on to the next barrier of the four warps)
+            if (!alive) break;
             uint8_t *K = base + 2 * L::Q + s * (L::K + L::V), *V = K + L::K;
-            if (w4 == 0 && lane < PG) sm.pos[j & 7][lane] = pos_here;
 #pragma unroll
             for (int i = 0; i < KI; i++) {
                 const int row = i * 4 * KROWS + k_row;
@@ -473,7 +498,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             fence_async_smem();
             mbar_arrive(smem_u32(&sm.k_full[s]));
             alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), ((j >> 1) & 1) ^ 1, flag));
-            if (!alive) continue;
+            if (!alive) break;
             {
                 uint32_t odd = 0;
 #pragma unroll
@@ -516,10 +541,48 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             fence_async_smem();
             mbar_arrive(smem_u32(&sm.v_full[s]));
         }
-        // a copy in flight after a wait that ran out ends before the CTA does
-        if (in_flight && nj > 0) {
-            for (int phase = 0; phase < 2; phase++) mbar_wait_quiet(smem_u32(&sm.raw_full), phase);
+    } else if (warp == 14) {
+        // ================= copies of the cache tiles
+        const int page_tiles = 1 << (A.shift - 4);
+        const uint32_t raw0 = smem_u32(base + 2 * L::Q + 2 * (L::K + L::V)), bar = smem_u32(&sm.raw_full);
+        // lane i < 8: cache tile i of position tile j and the page it lies on, used a position tile later (worked
+        // on at once, the load's latency stood in every tile)
+        int tile_next, page_next;
+        auto look = [&](int j) {
+            const int u = PG * j + (lane & 7);
+            tile_next = u < S.units ? S.tile(u) : 0;
+            page_next = u < S.units ? table[tile_next >> (A.shift - 4)] : -1;
+        };
+        // where it lies, or -1; and its first position
+        auto place = [&](int &pos) {
+            const bool there = page_next >= 0 && page_next < A.pages;
+            pos = there ? tile_next * KV4_TILE : ABSENT;
+            return there ? (int)(((int64_t)page_next * A.n_kv + kvh) * page_tiles + (tile_next & (page_tiles - 1))) : -1;
+        };
+        look(0);
+        int issued = 0;
+        for (; issued < nj; issued++) {
+            if (issued > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.raw_free), (issued - 1) & 1, flag))) break;
+            int pos;
+            const int at = place(pos);
+            // (the positions of eight tiles ago: the warps that read the raw tiles just now waited for their PV)
+            if (lane < PG) sm.pos[issued & 7][lane] = pos;
+            __syncwarp();
+            const int n = __popc(__ballot_sync(0xffffffffu, lane < PG && at >= 0));
+            if (lane == 0)
+                asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n}\n" ::"r"(bar),
+                             "r"(n * kv4_tile_bytes(HD))
+                             : "memory");
+            __syncwarp();
+            if (lane < PG && at >= 0)
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                 raw0 + lane * L::RAW1),
+                             "l"(A.cache + (uint64_t)(uint32_t)at * kv4_tile_bytes(HD)), "r"(kv4_tile_bytes(HD)), "r"(bar)
+                             : "memory");
+            look(issued + 1);
         }
+        // the last copy ends before the CTA does, also after a wait that ran out
+        if (issued > 0) mbar_wait_quiet(bar, (issued - 1) & 1);
     } else if (lane == 0) {
         // ================= MMAs: warp 12 S, warp 13 PV
         constexpr uint32_t id_s = idesc_f16(PN), id_o = idesc_f16(HD);
@@ -553,9 +616,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
 #pragma unroll
                 for (int ks = 0; ks < PN / 16; ks++) {
                     const uint64_t bd = vdesc + (((ks >> 2) * (HD * 128) + (ks & 3) * 32) >> 4);
-                    const uint32_t a = p0 + 32 * (ks >> 1) + 8 * (ks & 1);
+                    const uint32_t a = p0 + (CW == 32 ? 32 * (ks >> 1) + 8 * (ks & 1) : 16 * ks);
                     mma_ts(d, a, bd, id_o, ks > 0);
-                    mma_ts(d, a + 16, bd, id_o, 1);
+                    mma_ts(d, a + CW / 2, bd, id_o, 1);
                 }
                 commit(smem_u32(&sm.pv_done[s]));
                 mbar_arrive(smem_u32(&sm.pv_done[s]));         // (hands on the bit masks of the unpacking warps)
