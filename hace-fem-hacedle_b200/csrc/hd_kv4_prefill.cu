@@ -41,9 +41,9 @@
 // and P, 46% of the measured bf16 rate; chunks of 1 to 500 rows of 12 requests,
 // 14 heads on 2 of 64, 46.6 us.  What bounds it: the softmax warps and the
 // unpacking warps each take about 4.5 thousand cycles for 128 positions, the
-// MMAs 2.2 thousand.  No pipe is full (issue slots 52%, ALU 35%); after fixed
-// latencies the waits are for instructions, since either role runs through
-// its code once a tile.  Slower: 8 unpacking or 16 softmax warps (1.1 and 1.5
+// MMAs 2.2 thousand.  No pipe is full (issue slots 51%, tensor 36%): three
+// warps per scheduler wait for their own latencies, tensor memory's and the
+// instruction cache's (either role runs through its code once a tile).  Slower: 8 unpacking or 16 softmax warps (1.1 and 1.5
 // ms), registers moved from the issuing to the softmax warps (no spills, 1.1
 // ms), half of the scores kept in registers over the barrier (1.1 ms), the
 // unpacking loops rolled (1.03 ms).
