@@ -541,15 +541,15 @@ __global__ void __launch_bounds__(DNT, D_OCC) k_kv4_decode(Kv4Args A, int groups
             }
         }
         if (!alone) {
-            // pieces join in aligned groups of DJOIN CTAs first, whose sums then join, each by whoever comes last
-            const int g0 = (int)blockIdx.x / DJOIN, gb = max(first_cta, g0 * DJOIN), ge = min(last_cta, g0 * DJOIN + DJOIN - 1);
-            const int f0 = first_cta / DJOIN, ng = last_cta / DJOIN - f0 + 1;
+            // pieces join in groups of DJOIN CTAs first, whose sums then join, each by whoever comes last
+            const int gb = first_cta + ((int)blockIdx.x - first_cta) / DJOIN * DJOIN, ge = min(last_cta, gb + DJOIN - 1);
+            const int ng = (last_cta - first_cta) / DJOIN + 1;
             if (arrive(sm, tickets + slot_of(gb, first_cta), ge - gb)) {
                 join_parts<HD>(sm, parts, ml, ge - gb + 1, [&](int i) { return slot_of(gb + i, first_cta); }, nh,
                                ng > 1 ? slot_of(gb, first_cta) : -1, out);
                 if (ng > 1 && arrive(sm, tickets + 2 * gridDim.x + first_cta, ng - 1))
                     join_parts<HD>(sm, parts, ml, ng,
-                                   [&](int i) { return slot_of(max(first_cta, (f0 + i) * DJOIN), first_cta); }, nh, -1, out);
+                                   [&](int i) { return slot_of(first_cta + i * DJOIN, first_cta); }, nh, -1, out);
             }
         }
         __syncthreads();
