@@ -26,10 +26,12 @@
 // the output; pieces go to the workspace and the CTA that arrives last joins
 // them in order, so results do not depend on the schedule.  Many pieces of one
 // head (a long request alone) join in groups of 16 CTAs first, so that no CTA
-// walks hundreds of pieces alone.
+// walks hundreds of pieces alone; the groups count from the item's first CTA,
+// so that up to 16 pieces join once (32 requests with a window of 2048, 14
+// heads on 2 of 64: 12.6 us, 15.1 with groups of fixed CTAs).
 //
 // Measured, 28 heads on 4 kv heads of 128: 256 requests of 64 to 4096 tokens
-// (152 MB of cache) 66 us, 2.3 TB/s; one request of 131001 tokens (75 MB) 38 us,
+// (152 MB of cache) 65 us, 2.3 TB/s; one request of 131001 tokens (75 MB) 38 us,
 // 2.0 TB/s.  What bounds it is unpacking, not memory: about 440
 // instructions per warp and 16 positions at HD 128, of which the f16 ones go
 // at half rate, and the MMAs, together some 950 cycles a tile and SM sub-core
@@ -49,7 +51,7 @@ constexpr int DNT = 32 * DW;
 constexpr int DPT = 2;          // tiles per step
 template <int HD>
 constexpr int d_stages() { return HD == 128 ? 2 : HD == 64 ? 3 : 4; }   // steps in a warp's ring
-constexpr int DMIN = DPT * DW;  // fewest tiles a CTA takes
+constexpr int DMIN = DPT * DW;  // fewest tiles a CTA takes (32: 10.2 us for one request of 700 tokens, 8.4 with 8)
 constexpr int DHEADS = 8;       // query heads per unit
 constexpr int DCOST = 16;       // what beginning an item costs, in tiles (24: 3% slower over ragged lengths)
 constexpr int DJOIN = 16;       // CTAs whose partials are joined first

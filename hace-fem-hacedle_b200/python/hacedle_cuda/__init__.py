@@ -334,7 +334,7 @@ class Context:
         if _I32 is None:
             _dtypes()
         _dense(_U8, cache)
-        if cache.dim() != 4 or cache.shape[3] % 18:
+        if cache.dim() != 4 or cache.shape[3] % 18 or not cache.shape[3]:
             raise ValueError("cache must be [pages, n_kv, page_size / 16, 18 * head_dim]")
         pages, n_kv, tiles, width = cache.shape
         return pages, 16 * tiles, n_kv, width // 18

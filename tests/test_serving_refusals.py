@@ -111,6 +111,7 @@ def test_the_binding_refuses_tensors_that_do_not_fit():
         lambda: ctx.kv4_attention_decode(q, cache, i32(3, 4), i32(3), out[:2]),
         lambda: ctx.kv4_attention_decode(q.double(), cache, i32(3, 4), i32(3), out),
         lambda: ctx.kv4_attention_decode(q, cache[:, :, ::1, :17], i32(3, 4), i32(3), out),
+        lambda: ctx.kv4_attention_decode(q, cache[..., :0], i32(3, 4), i32(3), out),
         lambda: ctx.kv4_attention_prefill(q, cache, i32(2, 4), i32(2), i32(2), out),
         lambda: ctx.sample_filtered(torch.zeros(2, 50), torch.zeros(3), i32(2)),
         lambda: ctx.sample_filtered(torch.zeros(2, 50), torch.zeros(2), i32(2), top_k=torch.zeros(2)),
