@@ -432,11 +432,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
         const int v_word = HD == 128 ? 2 * (vr >> 3) : HD == 64 ? vr >> 2 : (vr >> 1) & 3;
         const bool v_on = HD != 32 || vr < 8;
         const uint8_t *raw0 = base + 2 * L::Q + 2 * (L::K + L::V);
-        bool alive = true;
         for (int j = 0; j < nj; j++) {
             const int s = j & 1;
-            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.raw_full), j & 1, flag));
-            if (!alive) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.raw_full), j & 1, flag))) break;
             const int pos = sm.pos[j & 7][lane & (PG - 1)];
             // whether every position is seen by some row (else the scales of the others count as 0)
             const bool whole = __all_sync(0xffffffffu, pos + KV4_TILE - 1 <= S.last && (pos >= S.first || pos <= A.sinks - KV4_TILE));
@@ -479,8 +477,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sm.raw_free));   // this warp has read the raw tiles
             // K's stage is free once the S that read it is there, V's once the PV is
-            alive = alive && __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.s_full[s]), ((j >> 1) & 1) ^ 1, flag));
-            if (!alive) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.s_full[s]), ((j >> 1) & 1) ^ 1, flag))) break;
             uint8_t *K = base + 2 * L::Q + s * (L::K + L::V), *V = K + L::K;
 #pragma unroll
             for (int i = 0; i < KI; i++) {
@@ -497,8 +494,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             }
             fence_async_smem();
             mbar_arrive(smem_u32(&sm.k_full[s]));
-            alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), ((j >> 1) & 1) ^ 1, flag));
-            if (!alive) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.pv_done[s]), ((j >> 1) & 1) ^ 1, flag))) break;
             {
                 uint32_t odd = 0;
 #pragma unroll

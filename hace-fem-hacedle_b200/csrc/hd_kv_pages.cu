@@ -16,9 +16,12 @@
 // One launch: every CTA of one cluster scans all requests (a few KB that the
 // L2 holds), and the cluster's threads share the rows.  The barrier of the
 // cluster stands between the last read of lens / n_free and the first write
-// of lens_out / n_free_out, which may be the same arrays.  The call moves 8
+// of lens_out / n_free_out, which may be the same arrays.  A step that only
+// decodes (up to 512 requests, a token each at most) is placed request by
+// request: no search, and the table entry is on its way during the scan (4.6 us
+// for the kernel alone, caches cold, 8.7 without).  The call moves 8
 // bytes a row; what bounds it is the latency of launch, loads and scan (7.2 us
-// a call from Python for a decode step of 256 requests, 7.9 for 1024 requests
+// a call from Python for a decode step of 256 requests, 8.2 for 1024 requests
 // with 96 chunks of prompts; a launch that does nothing takes 2.5).
 #include "hd_internal.cuh"
 #include "hd_mma.cuh"
@@ -88,27 +91,64 @@ __global__ void __launch_bounds__(PNT) k_pages_assign(const int32_t *lens, const
     pdl_trigger();
     const int tid = threadIdx.x, page = 1 << shift;
     const int per = (reqs + PNT - 1) / PNT, b = min(reqs, tid * per), e = min(reqs, b + per);
-    int64_t rows = 0, got = 0;
-    bool bad = false;
-    for (int r = b; r < e; r++) {
-        const int64_t l = lens[r], n = nnew[r];
-        if (l < 0 || n < 0 || l + n > (int64_t)max_pages << shift) {
-            bad = true;
-            break;
-        }
-        rows += n;
-        got += pages_of((int)(l + n), shift) - pages_of((int)l, shift);
-    }
     const int have_free = *n_free;
-    int64_t trows, tpages, arow = rows, apage = got;
-    scan2(arow, apage, trows, tpages);
-    bad = __syncthreads_or(bad);
-    const int st = bad || have_free < 0 || have_free > free_cap ? PAGES_BAD_REQUEST
-                   : tpages > have_free                         ? PAGES_SHORT
-                   : trows > max_rows                           ? PAGES_ROWS
-                                                                : PAGES_OK;
+    int64_t rows = 0, got = 0;
+    bool bad = false, many = false;
+    int id = -1;                       // the page that a single request's first new token lies on, if it is held
     for (int r = b; r < e; r++) {
-        const int l = lens[r], n = st == PAGES_OK ? nnew[r] : 0;
+        const int l = lens[r], n = nnew[r];
+        const bool wrong = l < 0 || n < 0 || (int64_t)l + n > (int64_t)max_pages << shift;
+        ln[r] = l;
+        r0[r] = n;
+        bad |= wrong;
+        many |= n > 1;
+        rows += wrong ? 0 : n;
+        got += wrong ? 0 : pages_of((int)((unsigned)l + (unsigned)n), shift) - pages_of(l, shift);
+    }
+    if (per == 1 && b < e && !bad && r0[b] > 0 && (ln[b] & (page - 1))) id = tables[(int64_t)b * max_pages + (ln[b] >> shift)];
+    __shared__ uint32_t flags[PNT / 32];
+    const uint32_t mine = __reduce_or_sync(0xffffffffu, (bad ? 1u : 0u) | (many ? 2u : 0u));
+    if ((tid & 31) == 0) flags[tid >> 5] = mine;
+    int64_t trows, tpages, arow = rows, apage = got;
+    scan2(arow, apage, trows, tpages);             // (its barrier is the flags', too)
+    const uint32_t seen = __reduce_or_sync(0xffffffffu, (tid & 31) < PNT / 32 ? flags[tid & 31] : 0u);
+    const bool any_bad = seen & 1, runs = seen & 2 || per > 1;
+    const int st = any_bad || have_free < 0 || have_free > free_cap ? PAGES_BAD_REQUEST
+                   : tpages > have_free                             ? PAGES_SHORT
+                   : trows > max_rows                               ? PAGES_ROWS
+                                                                    : PAGES_OK;
+    const int64_t me = (int64_t)blockIdx.x * PNT + tid, all = (int64_t)gridDim.x * PNT;
+    if (__builtin_expect(st == PAGES_OK && !runs, 0)) {
+        // a decode step (no request brings more than one token, no thread has two): each thread places its own
+        if (gridDim.x > 1) {           // every CTA of the cluster has read lens and n_free
+            mm_cluster_arrive_release();
+            mm_cluster_wait();
+        }
+        if (blockIdx.x == 0) {
+            if (tid == 0) {
+                row0[reqs] = (int)trows;
+                *n_free_out = have_free - (int)tpages;
+                *status = st;
+            }
+            if (b < e) {
+                const int l = ln[b], n = r0[b];
+                row0[b] = (int)arow;
+                lens_out[b] = l + n;
+                if (n) {
+                    if (!(l & (page - 1))) {
+                        id = free_list[have_free - 1 - (int)apage];
+                        tables[(int64_t)b * max_pages + (l >> shift)] = id;
+                    }
+                    slots[arow] = id >= 0 && id < pages ? (id << shift) + (l & (page - 1)) : -1;
+                    pos[arow] = l;
+                }
+            }
+        }
+        for (int64_t t = trows + me; t < max_rows; t += all) slots[t] = pos[t] = -1;
+        return;
+    }
+    for (int r = b; r < e; r++) {
+        const int l = ln[r], n = st == PAGES_OK ? r0[r] : 0;
         r0[r] = st == PAGES_OK ? (int)arow : 0;
         p0[r] = st == PAGES_OK ? (int)apage : 0;
         ln[r] = l;
@@ -120,11 +160,11 @@ __global__ void __launch_bounds__(PNT) k_pages_assign(const int32_t *lens, const
         r0[reqs] = (int)trows;
         p0[reqs] = (int)tpages;
     }
-    // every CTA of the cluster has read lens and n_free
-    mm_cluster_arrive_release();
-    mm_cluster_wait();
+    if (gridDim.x > 1) {               // every CTA of the cluster has read lens and n_free
+        mm_cluster_arrive_release();
+        mm_cluster_wait();
+    }
     __syncthreads();
-    const int64_t me = (int64_t)blockIdx.x * PNT + tid, all = (int64_t)gridDim.x * PNT;
     for (int64_t r = me; r <= reqs; r += all) {
         row0[r] = r0[r];
         if (r < reqs) lens_out[r] = ln[r] + (r0[r + 1] - r0[r]);
