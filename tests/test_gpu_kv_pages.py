@@ -40,7 +40,8 @@ def _run(ctx, torch, page, pages, lens, new, tables, free, rows, n_free=None, in
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("reqs,page,max_len,max_new,extra", [
     (1, 16, 0, 1, 0), (1, 16, 16, 1, 5), (1, 1024, 1023, 2, 0), (3, 16, 40, 17, 2), (33, 32, 100, 1, 0), (511, 16, 300, 3, 9),
-    (513, 64, 700, 40, 1), (1500, 16, 90, 30, 3), (8192, 16, 33, 2, 0), (2, 128, 5, 60000, 11), (40, 16, 0, 0, 4)])
+    (513, 64, 700, 40, 1), (1500, 16, 90, 30, 3), (8192, 16, 33, 2, 0), (2, 128, 5, 60000, 11), (40, 16, 0, 0, 4),
+    (512, 32, 500, 1, 20000), (513, 32, 500, 1, 20000)])
 def test_assign_matches_the_plain_loop(ctx, reqs, page, max_len, max_new, extra, in_place):
     import torch
     rng = np.random.default_rng(reqs + page)
