@@ -818,14 +818,48 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_sample_filtered(const float *
     }
 }
 
+constexpr int64_t HALF = 19456;              // elements of a slice of which two fit an SM
+template <int NT, bool RESIDENT>
+cudaError_t allow(const hd_ctx *ctx) {
+    static std::atomic<uint64_t> allowed{0};
+    return hd_allow_smem(allowed, ctx, (const void *)k_sample_filtered<NT, RESIDENT>,
+                         sizeof(FShared) + 16 + (RESIDENT ? FULL * sizeof(float) : 0), true);
+}
+
+// Clusters of 2^c CTAs with slices of up to HALF that the device runs at a
+// time; a cluster lies within one GPC, so these are fewer than the SMs allow.
+template <int NT>
+int at_a_time(const hd_ctx *ctx, int c) {
+    static std::atomic<int> known[64][8];    // 0: not asked yet
+    const bool keep = ctx->device < 64 && c < 8;
+    const int before = keep ? known[ctx->device][c].load(std::memory_order_relaxed) : 0;
+    if (before) return before - 1;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1u << c;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(1u << c);
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = sizeof(FShared) + 16 + HALF * sizeof(float);
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (allow<NT, true>(ctx) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, k_sample_filtered<NT, true>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (keep) known[ctx->device][c].store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+
 template <int NT, bool RESIDENT>
 cudaError_t launch(hd_ctx *ctx, int C, int64_t rows, int64_t slice, const float *logits, int64_t ld, int64_t n,
                    const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p, const float *u,
                    double unit, int half, int32_t *idx) {
     const size_t smem = (sizeof(FShared) + 15) / 16 * 16 + (RESIDENT ? (size_t)slice * sizeof(float) : 0);
     auto kernel = k_sample_filtered<NT, RESIDENT>;
-    static std::atomic<uint64_t> allowed{0};
-    cudaError_t e = hd_allow_smem(allowed, ctx, (const void *)kernel, sizeof(FShared) + 16 + (RESIDENT ? FULL * sizeof(float) : 0), true);
+    cudaError_t e = allow<NT, RESIDENT>(ctx);
     if (e != cudaSuccess) return e;
     const int wide = ((uintptr_t)logits & 15) == 0 && ld % 4 == 0;
     return hd_launch_cluster(ctx, kernel, dim3((unsigned)(rows * C)), dim3(NT), smem, C, logits, ld, n, temperature, top_k,
@@ -845,12 +879,25 @@ extern "C" int hd_sample_filtered(hd_ctx *ctx, const float *logits, int64_t ld, 
     if (!ctx) return HD_E_ARG;
     if (rows == 0) return HD_OK;
     HdDevice on(ctx);
-    // CTAs per row: as few as keep a slice at 80 KB, so that two CTAs share an SM; more while the rows
-    // alone leave SMs idle and a slice keeps 2048 elements
-    constexpr int64_t HALF = 19456;
+    // CTAs per row, and their threads.  A row's steps are the quicker the more of them (151936 logits, all rows at
+    // a time: 16 CTAs of 1024 threads 31 us, 8 of 1024 33, 16 of 512 35, 8 of 512 46), while slices keep 2048
+    // elements, but rows in a second wave cost as much again (8 rows: 56 us with 16 CTAs, 33 with 8).  So: the first
+    // of these that runs all rows at a time; with more rows than any of them, as few CTAs as keep two slices on an
+    // SM.
     auto slice_of = [&](int c) { return ((n + c - 1) / c + 3) / 4 * 4; };
-    int C = 1;
-    while (C < MAXC && (slice_of(C) > HALF || (rows * C < ctx->sm_count && slice_of(C) > 4096))) C *= 2;
+    int least = 0, most;                     // log2 of the CTAs
+    while ((1 << least) < MAXC && slice_of(1 << least) > HALF) least++;
+    for (most = least; (1 << most) < MAXC && slice_of(1 << most) > 4096;) most++;
+    int C = 0;
+    bool few = true;
+    for (int c = most; c >= least && !C; c--)
+        if (rows <= at_a_time<1024>(ctx, c)) C = 1 << c;
+    if (!C) {
+        few = false;
+        for (int c = most; c >= least && !C; c--)
+            if (rows <= at_a_time<512>(ctx, c)) C = 1 << c;
+        if (!C) C = 1 << least;
+    }
     const int64_t slice = slice_of(C);
     // Units: n of them sum below 2^62, and a lane's share of a resident slice times half of their bits below 2^32.
     auto log2_up = [](int64_t v) {
@@ -863,7 +910,6 @@ extern "C" int hd_sample_filtered(hd_ctx *ctx, const float *logits, int64_t ld, 
     if (slice <= FULL && bits > room) bits = room;
     const int half = (bits + 1) / 2;
     const double unit = std::ldexp(1.0, bits);
-    const bool few = rows * C <= ctx->sm_count;   // one CTA an SM: twice the threads
 #define HD_SAMPLE(NT, RES) launch<NT, RES>(ctx, C, rows, slice, logits, ld, n, temperature, top_k, top_p, min_p, u, unit, half, idx)
     cudaError_t e = slice > FULL ? HD_SAMPLE(1024, false) : few ? HD_SAMPLE(1024, true) : HD_SAMPLE(512, true);
 #undef HD_SAMPLE

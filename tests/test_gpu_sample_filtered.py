@@ -58,6 +58,17 @@ def test_matches_the_model(ctx, rows, n, kw):
     _check(ctx, torch, x, rng.random(rows).astype(np.float32), on_border=2 if kw.get("top_p") == 0.99999 and n > 100000 else 1, **kw)
 
 
+@pytest.mark.parametrize("rows,n", [(8, 151936), (20, 100000), (16, 20001), (40, 9001), (70, 20000), (300, 5000)])
+def test_rows_that_fill_the_machine_in_every_way(ctx, rows, n):
+    """Each number of CTAs and threads per row that the number of rows asks for."""
+    import torch
+    rng = np.random.default_rng(n + rows)
+    x = (rng.standard_normal((rows, n)) * 2.5).astype(np.float32)
+    u = rng.random(rows).astype(np.float32)
+    one = _check(ctx, torch, x, u, on_border=1, top_k=1000, top_p=0.9)
+    assert np.array_equal(_check(ctx, torch, x[:1], u[:1], on_border=1, top_k=1000, top_p=0.9), one[:1])
+
+
 @pytest.mark.parametrize("kw", SETTINGS, ids=str)
 def test_ties_go_to_the_lowest_index(ctx, kw):
     """Few distinct values: every threshold falls among equal logits."""
