@@ -20,6 +20,8 @@ struct Kv4Args {
     int n_heads, n_kv, window, sinks;
     float scale;
     float *out;
+    float scale_m;                // scale * log2(e) = scale_m * 2^scale_e, scale_m in [0.72, 1.45)
+    int scale_e;
 };
 
 // Refuses what the kernels do not take, and fills in shift and the defaults of

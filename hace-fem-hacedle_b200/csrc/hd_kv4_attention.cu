@@ -29,6 +29,7 @@ int hd_kv4_attention_check(hd_ctx *ctx, const char *name, Kv4Args &A, int page_s
                "%s: rows must be 16-byte aligned", name);
     if (!ctx) return HD_E_ARG;
     if (A.scale == 0.f) A.scale = 1.0f / sqrtf((float)hd);
+    A.scale_m = frexpf(A.scale, &A.scale_e) * 1.4426950408889634f;
     A.shift = 4;
     while ((1 << A.shift) < page_size) A.shift++;
     return HD_OK;

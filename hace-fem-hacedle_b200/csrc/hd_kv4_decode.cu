@@ -6,8 +6,8 @@
 // share it.  Both products run on m16n8k16 MMAs: rows 0..7 of the A operand
 // are the heads' high f16 parts and rows 8..15 their low parts, so one MMA
 // multiplies both and adding accumulator rows g and g + 8 -- which the same
-// thread holds -- gives 22 significant bits of q (scaled by a power of two per
-// head) and of the softmax weights (scaled by 2^15), against cache values that
+// thread holds -- gives 22 significant bits of q (scaled per
+// head) and of the softmax weights (the largest at 2^15), against cache values that
 // are exact in f16 (hd_kv4.cuh).  The score accumulators are already in the
 // layout the second product wants its A operand in.
 //
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(DNT, D_OCC) k_kv4_decode(Kv4Args A, int groups
         const int kvh = item / groups, h0 = (item - kvh * groups) * gh, nh = min(gh, rep - h0);
         const int32_t *table = A.tables + (int64_t)req * A.max_pages;
 
-        // ---- q of the heads, in two f16 parts scaled to 2^14 (one warp; the others wait below)
+        // ---- q of the heads, scaled, in two f16 parts (one warp; the others wait below)
         if (warp == 0) {
             float x[WPT][8];
             const float *q = A.q + (int64_t)req * A.q_ld + (int64_t)(kvh * rep + h0 + g) * HD;
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(DNT, D_OCC) k_kv4_decode(Kv4Args A, int groups
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             float up, kappa;
-            q_scales(mx, A.scale, up, kappa);
+            q_scales(A, mx, up, kappa);
             if (t == 0) sm.kappa[g] = kappa;
 #pragma unroll
             for (int w = 0; w < WPT; w++)
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(DNT, D_OCC) k_kv4_decode(Kv4Args A, int groups
         for (int s = 0; s < NS - 1; s++) fetch(s, s);
         __syncthreads();                // q is there
         const float kappa = sm.kappa[g];
-        float o[NT][4], m = -INFINITY, l = 0.f;
+        float o[NT][4], m = -INFINITY, ref = 0.f, l = 0.f;
 #pragma unroll
         for (int i = 0; i < NT; i++)
 #pragma unroll
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(DNT, D_OCC) k_kv4_decode(Kv4Args A, int groups
             for (int j = 0; j < DPT; j++) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    e[j][c] = (s[2 * j + (c >> 1)][c & 1] + s[2 * j + (c >> 1)][(c & 1) + 2]) * kappa;
+                    e[j][c] = s[2 * j + (c >> 1)][c & 1] + s[2 * j + (c >> 1)][(c & 1) + 2];
                 }
             }
             if (hidden) {
@@ -444,21 +444,21 @@ __global__ void __launch_bounds__(DNT, D_OCC) k_kv4_decode(Kv4Args A, int groups
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             if (__any_sync(0xffffffffu, mx > m)) {
-                const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : exp2_approx(m - mn);
+                const float mn = fmaxf(m, mx), rn = weight_ref(mn, kappa), a = m == -INFINITY ? 0.f : exp2_approx(ref - rn);
                 m = mn;
+                ref = rn;
                 l *= a;
 #pragma unroll
                 for (int i = 0; i < NT; i++)
 #pragma unroll
                     for (int c = 0; c < 4; c++) o[i][c] *= a;
             }
-            const float ref = m == -INFINITY ? 0.f : m - 15.f;
             uint32_t pa[DPT][4];
 #pragma unroll
             for (int j = 0; j < DPT; j++) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    e[j][c] = exp2_approx(e[j][c] - ref);
+                    e[j][c] = exp2_approx(fmaf(e[j][c], kappa, -ref));
                     l += e[j][c];
                 }
                 split2(e[j][0], e[j][1], pa[j][0], pa[j][1]);
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(DNT, D_OCC) k_kv4_decode(Kv4Args A, int groups
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (t == 0) {
-            sm.m[warp][g] = m;
+            sm.m[warp][g] = m == -INFINITY ? m : ref;   // what the warp's l and o are in units of
             sm.l[warp][g] = l;
         }
 #pragma unroll

@@ -57,14 +57,29 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// A row of q whose largest magnitude is mx is scaled by a power of two to
-// about 2^14 for its f16 parts: that factor, and what takes its scores to
-// base-2 exponents.
-__device__ __forceinline__ void q_scales(float mx, float scale, float &up, float &kappa) {
+// A row of q whose largest magnitude is mx is multiplied by `up` for its f16
+// parts, which takes that to between 2^13 and 2^16 (at most 47500); kappa, a
+// power of two, then takes its scores to base-2 exponents: the significant bits
+// of scale * log2(e) are in `up`, so s * kappa is exact.  |s| < 2^39 (128
+// products with cache values below 2^16), and kappa is held to 2^-120 .. 2^88,
+// so s * kappa is finite and -infinity * kappa is -infinity; at those ends
+// scores that differ at all are too far apart, or all too close, for kappa to
+// matter.
+__device__ __forceinline__ void q_scales(const Kv4Args &A, float mx, float &up, float &kappa) {
     int e = (int)(__float_as_uint(mx) >> 23) - 127;
-    e = e < -100 ? -100 : e;                // the factor and its inverse stay normal numbers
-    up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-    kappa = scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+    e = e < -100 ? -100 : e;                // the factor stays a normal number
+    up = A.scale_m * __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+    const int k = A.scale_e + e - 14;
+    kappa = __uint_as_float((uint32_t)(127 + (k < -120 ? -120 : k > 88 ? 88 : k)) << 23);
+}
+// Weights are 2^(s kappa - ref) with ref = m kappa - 15 rounded up, m the
+// largest score so far: the largest weight lies at 2^15 for its f16 parts, and
+// never above it, whatever the size of the scores.  (Rounded to nearest, from
+// |m kappa| = 2^24 on it came to 2^16, infinite in f16.)  Where a step of the
+// scores is 2 or more, weights are whole powers of two and their largest is at
+// least 1, so nothing is lost there either.
+__device__ __forceinline__ float weight_ref(float m, float kappa) {
+    return m == -INFINITY ? 0.f : __fmaf_ru(m, kappa, -15.f);
 }
 
 // The tiles that queries at positions i0 .. last of a request see: `sink`

@@ -273,8 +273,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
         sm.mx[0][half][r] = mx;
         bar_sync(1, P_SOFT);
         float up;
-        q_scales(fmaxf(sm.mx[0][0][r], sm.mx[0][1][r]), A.scale, up, kappa);
-        kappa = fmaxf(kappa, 1e-37f);                      // -infinity * kappa stays -infinity
+        q_scales(A, fmaxf(sm.mx[0][0][r], sm.mx[0][1][r]), up, kappa);
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int ch = half * CH + c;
@@ -373,10 +372,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
             sm.mx[s][half][r] = mx;          // (the other buffer next time: one barrier a tile is enough)
             bar_sync(1, P_SOFT);
             if (!alive) continue;
-            mx = fmaxf(mx, sm.mx[s][half ^ 1][r]) * kappa;
-            const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : exp2_approx(m - mn);
+            const float mn = fmaxf(m, fmaxf(mx, sm.mx[s][half ^ 1][r])), ref = weight_ref(mn, kappa);
+            const float a = m == -INFINITY ? 0.f : exp2_approx(weight_ref(m, kappa) - ref);
             m = mn;
-            const float ref = m == -INFINITY ? 0.f : m - 15.f;
             const uint64_t kappa2 = pack2(kappa, kappa), ref2 = pack2(-ref, -ref);
             uint64_t sum = 0;
 #pragma unroll 1
