@@ -38,10 +38,12 @@
 // Weights are computed in 64 bits (2^y = 2^(j/256) 2^e 2^r with a table of 256
 // and a polynomial of degree 4 in r, |r| <= 1/512: the table-driven method of
 // P. T. P. Tang, ACM TOMS 15 (1989), error below 2^-50) and held as whole
-// numbers of 2^-s, s = 40 to 50 by the length of the row (42 for a vocabulary
-// of 152k): sums are exact in any order, so neither atomics nor the shape of
-// the cluster can change a draw, and a weight's rounding is far below what
-// float32 sums lose.
+// numbers of 2^-s: sums are exact in any order, so neither atomics nor the
+// shape of the cluster can change a draw.  s follows from n alone: 50 up to
+// 2048 logits, 42 for a vocabulary of 152k, 40 at least up to 737280, then 62 -
+// log2(n) rounded up, 31 for the longest.  A weight is off by at most 2^-(s+1)
+// of the largest and a running sum by n times that: 1.7e-8 for 152k, below
+// what a float32 sum loses at one addition, and up to 0.5 for the longest.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -899,15 +901,17 @@ extern "C" int hd_sample_filtered(hd_ctx *ctx, const float *logits, int64_t ld, 
         if (!C) C = 1 << least;
     }
     const int64_t slice = slice_of(C);
-    // Units: n of them sum below 2^62, and a lane's share of a resident slice times half of their bits below 2^32.
+    // Units: n of them sum below 2^62, and a lane's share of a resident slice times half of their bits below 2^32.  The
+    // slice is the longest that any number of rows leads to, so that a row's weights are the same in every batch.
     auto log2_up = [](int64_t v) {
         int b = 0;
         while (((int64_t)1 << b) < v) b++;
         return b;
     };
     int bits = 62 - log2_up(n) < 50 ? 62 - log2_up(n) : 50;
-    const int room = 2 * (36 - log2_up(slice));
-    if (slice <= FULL && bits > room) bits = room;
+    const int64_t longest = slice_of(1 << least);
+    const int room = 2 * (36 - log2_up(longest));
+    if (longest <= FULL && bits > room) bits = room;
     const int half = (bits + 1) / 2;
     const double unit = std::ldexp(1.0, bits);
 #define HD_SAMPLE(NT, RES) launch<NT, RES>(ctx, C, rows, slice, logits, ld, n, temperature, top_k, top_p, min_p, u, unit, half, idx)

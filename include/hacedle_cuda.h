@@ -376,7 +376,11 @@ int hd_sample_rows(hd_ctx *ctx, const float *logits_dev, int64_t rows, int64_t n
  * sum of kept weights exceeds u times their sum (u outside [0, 1) is taken as
  * the nearest inside).  NaN logits count as -infinity, which is never drawn; a
  * row with nothing else gives -1.  ld: row stride of logits_dev in floats (0:
- * n).  n < 2^31.  Sums are exact, so a draw depends on its inputs alone. */
+ * n).  n < 2^31.  Weights are held as whole multiples of 2^-s (s from n alone:
+ * 50 up to 2048 logits, 42 for 152k, at least 40 up to 737280, then 62 -
+ * log2(n) rounded up) and their sums are exact, so a draw depends on its own
+ * row's inputs alone, whatever else is in the batch; a weight below half of
+ * 2^-s is never drawn. */
 int hd_sample_filtered(hd_ctx *ctx, const float *logits_dev, int64_t ld, int64_t rows, int64_t n,
                        const float *temperature_dev, const int32_t *top_k_dev, const float *top_p_dev,
                        const float *min_p_dev, const float *u_dev, int32_t *idx_dev);
