@@ -139,7 +139,7 @@ def _ptr(t) -> int | None:
 
 
 # The paged-cache and sampling calls are short on the GPU, so their checks are
-# kept to what a wrong tensor could break: type, density and size.
+# kept to what a wrong tensor could break: type, density, size and device.
 _I32 = _F32 = _U8 = None
 
 
@@ -150,10 +150,23 @@ def _dtypes():
     _I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 
 
-def _dense(dtype, *tensors):
+def _dense(device, dtype, *tensors) -> bool:
+    """Refuses tensors of another type or with gaps.  True if one lies on another device, which the
+    caller refuses (_elsewhere) once nothing else is wrong: one loop, since a loop of its own costs
+    a call of eleven tensors a quarter of a microsecond."""
+    away = False
     for t in tensors:
         if t.dtype is not dtype or not t.is_contiguous():
             raise ValueError(f"a dense {dtype} tensor is wanted, not {t.dtype} of strides {t.stride()}")
+        if t.get_device() != device:
+            away = True
+    return away
+
+
+def _elsewhere(device, *tensors):
+    """A kernel would take a host address, or another device's, for one of its own."""
+    other = [t.device for t in tensors if t is not None and t.get_device() != device]
+    raise ValueError(f"tensors on the context's device {device} are wanted, not one on {other[0]}")
 
 
 def _row_stride(t) -> int:
@@ -212,6 +225,8 @@ class Weight:
 
 class Context:
     """One hd_ctx on `device`; work goes on torch's current stream."""
+
+    device: int | None = None
 
     def __init__(self, device: int = 0, use_torch_stream: bool = True):
         import torch
@@ -280,19 +295,22 @@ class Context:
         if _I32 is None:
             _dtypes()
         rows, n = logits.shape
-        _dense(_F32, u)
-        _dense(_I32, idx)
+        dev = self.device
+        away = _dense(dev, _F32, u) | _dense(dev, _I32, idx) | (logits.get_device() != dev)
         bad = u.numel() != rows or idx.numel() != rows
         for t in (temperature, top_p, min_p):
             if t is not None:
-                _dense(_F32, t)
+                away |= _dense(dev, _F32, t)
                 bad = bad or t.numel() != rows
         if top_k is not None:
-            _dense(_I32, top_k)
+            away |= _dense(dev, _I32, top_k)
             bad = bad or top_k.numel() != rows
         if bad:
             raise ValueError(f"u, idx and the settings must have one entry for each of the {rows} rows")
-        rc = lib().hd_sample_filtered(self.h, logits.data_ptr(), _row_stride(logits), rows, n, _ptr(temperature), _ptr(top_k),
+        ld = _row_stride(logits)
+        if away:
+            _elsewhere(dev, logits, u, idx, temperature, top_k, top_p, min_p)
+        rc = lib().hd_sample_filtered(self.h, logits.data_ptr(), ld, rows, n, _ptr(temperature), _ptr(top_k),
                                       _ptr(top_p), _ptr(min_p), u.data_ptr(), idx.data_ptr())
         if rc:
             self._check(rc)
@@ -305,12 +323,14 @@ class Context:
         pos [max_rows]; n_free_out / lens_out may be n_free / lens."""
         if _I32 is None:
             _dtypes()
-        _dense(_I32, lens, new, tables, free, n_free, n_free_out, lens_out, row0, slots, pos, status)
+        away = _dense(self.device, _I32, lens, new, tables, free, n_free, n_free_out, lens_out, row0, slots, pos, status)
         reqs, width = tables.shape
         rows = slots.numel()
         if lens.numel() != reqs or new.numel() != reqs or lens_out.numel() != reqs or row0.numel() != reqs + 1 or \
                 rows != pos.numel():
             raise ValueError(f"lens, new, lens_out, row0, slots or pos do not fit {reqs} requests")
+        if away:
+            _elsewhere(self.device, lens, new, tables, free, n_free, n_free_out, lens_out, row0, slots, pos, status)
         rc = lib().hd_kv_pages_assign(self.h, lens.data_ptr(), new.data_ptr(), reqs, tables.data_ptr(), width, page_size, pages,
                                       free.data_ptr(), n_free.data_ptr(), free.numel(), n_free_out.data_ptr(), lens_out.data_ptr(),
                                       row0.data_ptr(), slots.data_ptr(), pos.data_ptr(), rows, status.data_ptr())
@@ -321,46 +341,55 @@ class Context:
         """Gives back the pages of the requests with done[r] != 0."""
         if _I32 is None:
             _dtypes()
-        _dense(_I32, done, lens, tables, free, n_free, status)
+        away = _dense(self.device, _I32, done, lens, tables, free, n_free, status)
         reqs, width = tables.shape
         if lens.numel() != reqs or done.numel() != reqs:
             raise ValueError(f"lens or done do not fit {reqs} requests")
+        if away:
+            _elsewhere(self.device, done, lens, tables, free, n_free, status)
         self._check(lib().hd_kv_pages_release(self.h, done.data_ptr(), lens.data_ptr(), reqs, tables.data_ptr(), width,
                                               page_size, free.data_ptr(), n_free.data_ptr(), free.numel(), status.data_ptr()))
 
-    @staticmethod
-    def _kv4_shape(cache):
-        """(pages, page_size, n_kv, head_dim) of a uint8 cache tensor [pages, n_kv, page_size / 16, 18 * head_dim]."""
+    def _kv4_shape(self, cache):
+        """(pages, page_size, n_kv, head_dim, whether it lies elsewhere) of a uint8 cache tensor
+        [pages, n_kv, page_size / 16, 18 * head_dim]."""
         if _I32 is None:
             _dtypes()
-        _dense(_U8, cache)
-        if cache.dim() != 4 or cache.shape[3] % 18 or not cache.shape[3]:
+        away = _dense(self.device, _U8, cache)
+        shape = cache.shape
+        if len(shape) != 4 or shape[3] % 18 or not shape[3]:
             raise ValueError("cache must be [pages, n_kv, page_size / 16, 18 * head_dim]")
-        pages, n_kv, tiles, width = cache.shape
-        return pages, 16 * tiles, n_kv, width // 18
+        pages, n_kv, tiles, width = shape
+        return pages, 16 * tiles, n_kv, width // 18, away
 
     def kv4_append(self, k, v, slots, cache):
         """k, v [rows, n_kv, head_dim] (rows may be strided) quantized into the cache's slots."""
-        pages, page, n_kv, hd = self._kv4_shape(cache)
-        _dense(_I32, slots)
+        pages, page, n_kv, hd, away = self._kv4_shape(cache)
+        dev = self.device
+        away |= _dense(dev, _I32, slots)
         rows = slots.numel()
         n = rows * n_kv * hd
         if k.shape[0] != rows or v.shape[0] != rows or k.numel() != n or v.numel() != n:
             raise ValueError("k, v, slots and cache do not fit")
-        rc = lib().hd_kv4_append(self.h, k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v), slots.data_ptr(), rows,
-                                 n_kv, hd, cache.data_ptr(), pages, page)
+        k_ld, v_ld = _row_stride(k), _row_stride(v)
+        if away or k.get_device() != dev or v.get_device() != dev:
+            _elsewhere(dev, k, v, slots, cache)
+        rc = lib().hd_kv4_append(self.h, k.data_ptr(), v.data_ptr(), k_ld, v_ld, slots.data_ptr(), rows, n_kv, hd,
+                                 cache.data_ptr(), pages, page)
         if rc:
             self._check(rc)
 
     def kv4_read(self, cache, slots, k, v):
         """The values that slots hold into k, v [rows, n_kv, head_dim]."""
-        pages, page, n_kv, hd = self._kv4_shape(cache)
-        _dense(_I32, slots)
-        _dense(_F32, k, v)
+        pages, page, n_kv, hd, away = self._kv4_shape(cache)
+        away |= _dense(self.device, _I32, slots)
+        away |= _dense(self.device, _F32, k, v)
         rows = slots.numel()
         n = rows * n_kv * hd
         if k.numel() != n or v.numel() != n:
             raise ValueError("k, v, slots and cache do not fit")
+        if away:
+            _elsewhere(self.device, cache, slots, k, v)
         rc = lib().hd_kv4_read(self.h, cache.data_ptr(), pages, page, slots.data_ptr(), rows, n_kv, hd, k.data_ptr(),
                                v.data_ptr())
         if rc:
@@ -369,30 +398,33 @@ class Context:
     def kv4_workspace_bytes(self, n_heads: int, n_kv: int, head_dim: int) -> int:
         return int(lib().hd_kv4_workspace_bytes(self.h, n_heads, n_kv, head_dim))
 
-    @staticmethod
-    def _kv4_heads(q, tables, lens, out, hd: int) -> int:
-        _dense(_I32, tables, lens)
-        _dense(_F32, out)
+    def _kv4_heads(self, q, tables, lens, out, hd: int):
+        """(query heads, row stride of q, whether a tensor lies elsewhere)."""
+        dev = self.device
+        away = _dense(dev, _I32, tables, lens)
+        away |= _dense(dev, _F32, out)
         rows, n = q.shape[0], q.numel()
         heads = n // (rows * hd)
         if tables.dim() != 2 or tables.shape[0] != lens.numel() or out.numel() != n or heads * rows * hd != n:
             raise ValueError("q, cache, tables, lens and out do not fit")
-        return heads
+        return heads, _row_stride(q), away or q.get_device() != dev
 
     def kv4_attention_decode(self, q, cache, tables, lens, out, window: int = 0, sinks: int = 0, scale: float = 0.0, ws=None):
         """q [seqs, heads, head_dim] (rows may be strided): each request's last
         position against its cached ones.  ws: a zeroed uint8 tensor of
         kv4_workspace_bytes, or None for the context's own."""
-        pages, page, n_kv, hd = self._kv4_shape(cache)
+        pages, page, n_kv, hd, cache_away = self._kv4_shape(cache)
         seqs = lens.numel()
         if q.shape[0] != seqs:
             raise ValueError("q must have one row for each request")
         if not seqs:
             return
-        heads = self._kv4_heads(q, tables, lens, out, hd)
+        heads, ld, away = self._kv4_heads(q, tables, lens, out, hd)
         if ws is not None:
-            _dense(_U8, ws)
-        rc = lib().hd_kv4_attention_decode(self.h, q.data_ptr(), _row_stride(q), cache.data_ptr(), pages, page,
+            away |= _dense(self.device, _U8, ws)
+        if away or cache_away:
+            _elsewhere(self.device, q, cache, tables, lens, out, ws)
+        rc = lib().hd_kv4_attention_decode(self.h, q.data_ptr(), ld, cache.data_ptr(), pages, page,
                                            tables.data_ptr(), tables.shape[1], lens.data_ptr(), seqs, heads, n_kv, hd, window,
                                            sinks, scale, out.data_ptr(), None if ws is None else ws.data_ptr(),
                                            0 if ws is None else ws.numel())
@@ -401,15 +433,17 @@ class Context:
 
     def kv4_attention_prefill(self, q, cache, tables, lens, row0, out, window: int = 0, sinks: int = 0, scale: float = 0.0):
         """q [rows, heads, head_dim]: rows row0[r] .. row0[r+1]-1 are request r's last positions."""
-        pages, page, n_kv, hd = self._kv4_shape(cache)
+        pages, page, n_kv, hd, cache_away = self._kv4_shape(cache)
         rows, seqs = q.shape[0], lens.numel()
         if not rows:
             return
-        heads = self._kv4_heads(q, tables, lens, out, hd)
-        _dense(_I32, row0)
+        heads, ld, away = self._kv4_heads(q, tables, lens, out, hd)
+        away |= _dense(self.device, _I32, row0)
         if row0.numel() != seqs + 1:
             raise ValueError("row0 must have one more entry than lens")
-        rc = lib().hd_kv4_attention_prefill(self.h, q.data_ptr(), _row_stride(q), cache.data_ptr(), pages, page,
+        if away or cache_away:
+            _elsewhere(self.device, q, cache, tables, lens, row0, out)
+        rc = lib().hd_kv4_attention_prefill(self.h, q.data_ptr(), ld, cache.data_ptr(), pages, page,
                                             tables.data_ptr(), tables.shape[1], lens.data_ptr(), row0.data_ptr(), seqs, rows,
                                             heads, n_kv, hd, window, sinks, scale, out.data_ptr())
         if rc:
