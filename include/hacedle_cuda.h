@@ -464,7 +464,9 @@ int hd_kv_pages_assign(hd_ctx *ctx, const int32_t *lens_dev, const int32_t *new_
                        int32_t *pos_dev, int64_t max_rows, int32_t *status_dev);
 /* Returns the pages of every request with done_dev[r] != 0 to the end of the
  * free stack (request order, table order), sets its length to 0 and its table
- * entries to -1.  free_cap: ids free_dev has room for.  status_dev: 0; 1: they
+ * entries to -1.  Held entries outside [0, 2^31 / page_size) name no page (one
+ * given back early behind a window, say) and are dropped; all others are taken
+ * to be pages of this pool.  free_cap: ids free_dev has room for.  status_dev: 0; 1: they
  * would not fit; 2: a length or the free count is out of range; with 1 and 2
  * nothing changes. */
 int hd_kv_pages_release(hd_ctx *ctx, const int32_t *done_dev, int32_t *lens_dev, int reqs, int32_t *tables_dev,
