@@ -243,7 +243,10 @@ class Context:
     def set_stream(self, stream: int | None):
         """Enqueue on `stream` (a cudaStream_t as int).  Handle 0, torch's
         default stream, is the legacy default stream: it is passed as
-        cudaStreamLegacy (1), because NULL selects the context's own stream."""
+        cudaStreamLegacy (1), because NULL selects the context's own stream.
+        The context's own workspaces (of split-K products, of
+        kv4_attention_decode without ws) go with it: order the new stream
+        behind the old one where calls on both use them."""
         self._check(lib().hd_ctx_set_stream(self.h, stream if stream else CUDA_STREAM_LEGACY))
 
     def _check(self, rc: int):
@@ -412,7 +415,8 @@ class Context:
     def kv4_attention_decode(self, q, cache, tables, lens, out, window: int = 0, sinks: int = 0, scale: float = 0.0, ws=None):
         """q [seqs, heads, head_dim] (rows may be strided): each request's last
         position against its cached ones.  ws: a zeroed uint8 tensor of
-        kv4_workspace_bytes, or None for the context's own."""
+        kv4_workspace_bytes, or None for the context's own; calls that may run
+        at the same time (another stream, another graph) need one each."""
         pages, page, n_kv, hd, cache_away = self._kv4_shape(cache)
         seqs = lens.numel()
         if q.shape[0] != seqs:

@@ -64,7 +64,13 @@ int hd_ctx_create(int device, hd_ctx **out);
 int hd_ctx_destroy(hd_ctx *ctx);
 /* Enqueue subsequent work on `stream` (a cudaStream_t); NULL restores the
  * context's own (non-blocking) stream.  Pass cudaStreamLegacy for the legacy
- * default stream. */
+ * default stream.  Nothing is waited for, and the context's own workspaces
+ * (split-K partials and tickets, the argmax keys, the paged decode attention's
+ * when none is passed) go with it: where calls before and after the change use
+ * them, order the new stream behind the old one (an event, or
+ * hd_ctx_synchronize before the change), or use a context per stream.  The same
+ * holds for graphs captured from one context that may be replayed at the same
+ * time. */
 int hd_ctx_set_stream(hd_ctx *ctx, void *stream);
 int hd_ctx_synchronize(hd_ctx *ctx);
 /* Make sure the context's split-K workspace holds at least `bytes`, so that
@@ -509,8 +515,10 @@ int hd_kv4_read(hd_ctx *ctx, const uint8_t *cache_dev, int64_t pages, int page_s
  * decode:  row r is request r's last position, lens_dev[r] - 1.
  *          ws_dev: hd_kv4_workspace_bytes bytes (16-byte aligned), zeroed once
  *          before their first use; calls that may run at the same time (two
- *          streams, two graphs) need one each.  NULL: the context's own, made by
- *          its first such call, which must not be captured.
+ *          streams, two graphs) need one each, else their results are
+ *          undefined.  NULL: the context's own, made by its first such call,
+ *          which must not be captured (hd_ctx_set_stream says what a change of
+ *          stream asks then).
  * prefill: rows row0[r] .. row0[r+1]-1 are the last positions of request r
  *          (row0_dev [seqs + 1] ascending from 0, row0[seqs] <= rows); rows: of
  *          q and out; those from row0[seqs] on are left as they are.  A request's
