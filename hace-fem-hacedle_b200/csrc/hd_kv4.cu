@@ -20,9 +20,10 @@ __device__ __noinline__ uint32_t quant4_exact(float a, float b, float c, float e
 // value that has it by a vote, the nibbles of the upper half passed to the
 // threads that hold the lower half, and 16 bytes written by two threads.
 //
-// 16383 rows of 2 x 4 x 128 values take 26 us (76 MB; 11.7 us at the measured
-// copy rate): instruction issue, 58% of its slots busy, bounds it before the
-// rows read do (4 bytes a value against 0.56 written).  The first form (four
+// 16383 rows of 2 x 4 x 128 values take 22 us a call among others of its kind,
+// 25 with cold caches (76 MB; 11.7 us at the measured copy rate): instruction
+// issue, 72% of its slots busy, bounds it before the rows read do (4 bytes a
+// value against 0.56 written).  The first form (four
 // values a thread, 64-bit indices, the exact rounding of every value) took 337
 // instructions a thread and 53 us; here the exact comparison is left to values
 // within 10^-5 of a tie.

@@ -38,15 +38,20 @@
 //
 // Measured: 4096 rows on 8192 positions, 28 heads on 4 of 128 (361 GFLOP
 // counted once), 0.94 ms: 384 TFLOP/s, 769 of MMA work with the two parts of q
-// and P, 46% of the measured bf16 rate; chunks of 1 to 500 rows of 12 requests,
-// 14 heads on 2 of 64, 46.6 us.  What bounds it: the softmax warps and the
-// unpacking warps each take about 4.5 thousand cycles for 128 positions, the
-// MMAs 2.2 thousand.  No pipe is full (issue slots 51%, tensor 36%): three
-// warps per scheduler wait for their own latencies, tensor memory's and the
-// instruction cache's (either role runs through its code once a tile).  Slower: 8 unpacking or 16 softmax warps (1.1 and 1.5
-// ms), registers moved from the issuing to the softmax warps (no spills, 1.1
-// ms), half of the scores kept in registers over the barrier (1.1 ms), the
-// unpacking loops rolled (1.03 ms).
+// and P, 46% of the measured bf16 rate.  What bounds that: an SM takes 299 steps
+// of 128 positions, 6.2 thousand cycles each, where the softmax warps or the
+// unpacking warps alone need about 4.5 thousand and the MMAs 2.2 thousand, so
+// the roles wait for one another as well.  No pipe is full (issue slots 51%,
+// tensor 36%): three warps per scheduler wait for their own latencies, tensor
+// memory's and the instruction cache's (either role runs through its code once
+// a tile).  Chunks of 1 to 500 rows of 12 requests, 14 heads on 2 of 64, take 37
+// to 47 us by how long the chunks' prefixes are: 154 CTAs are about one wave,
+// and the one with the longest walk (16 to 18 steps, 2.4 to 6 on average) sets
+// the time, since a row tile's positions are not split.  Slower: 8 unpacking or
+// 16 softmax warps (1.1 and 1.5 ms), registers moved from the issuing to the
+// softmax warps (no spills, 1.1 ms), half of the scores kept in registers over
+// the barrier (1.1 ms), the unpacking loops rolled (1.03 ms), a subtraction of
+// the maximum before the multiplication with kappa (0.96 ms).
 #include "hd_internal.cuh"
 #include "hd_kv4_math.cuh"
 #include "hd_tc.cuh"

@@ -18,11 +18,13 @@
 // cluster stands between the last read of lens / n_free and the first write
 // of lens_out / n_free_out, which may be the same arrays.  A step that only
 // decodes (up to 512 requests, a token each at most) is placed request by
-// request: no search, and the table entry is on its way during the scan (4.6 us
-// for the kernel alone, caches cold, 8.7 without).  The call moves 8
-// bytes a row; what bounds it is the latency of launch, loads and scan (7.2 us
-// a call from Python for a decode step of 256 requests, 8.2 for 1024 requests
-// with 96 chunks of prompts; a launch that does nothing takes 2.5).
+// request: no search, and the table entry is on its way during the scan (4.4 us
+// for the kernel alone, caches cold, 8.7 without; a step of 1024 requests, 96 of
+// which bring chunks, takes the other way: 11.1).  The call moves 8 bytes a row;
+// what bounds it is the latency of loads and scan, and from Python the binding
+// (7.8 us a call for a decode step of 256 requests, of which the checks of eleven
+// tensors' devices are 0.5, and 8.1 for the step with chunks; a launch that does
+// nothing takes 2.5).
 #include <climits>
 
 #include "hd_internal.cuh"
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(PNT) k_pages_assign(const int32_t *lens, const
 // order.  Entries below 0 (pages given back early behind a window) or beyond
 // what any cache of fewer than 2^31 slots has name none: on the stack they
 // would be dealt to another request, whose tokens would then have no slot.
-// A call among others takes 6.0 us for 1695 pages of 13 requests out of 256, 14
+// A call among others takes 6.0 us for 1695 pages of 14 requests out of 256, 14
 // for 6977 (16 with one entry a thread at a time), 219 for 193834: a search and
 // a load in turn, on one SM, bound it.
 __global__ void __launch_bounds__(PNT) k_pages_release(const int32_t *__restrict__ done, int32_t *lens, int reqs,

@@ -26,13 +26,12 @@
 // time (4: 1.5 us more per row), and the search for a bin's bounds tries the
 // keys next to the computed one first (1.2 us less).
 //
-// 256 rows of 151936 logits with top-p 0.95 take 0.32 ms (156 MB: 24 us at the
-// measured copy rate), one row 31 us.  What bounds it: a row passes through
+// 256 rows of 151936 logits, most with top-p 0.95, take 0.285 ms (156 MB: 24 us
+// at the measured copy rate), one row 31 us.  What bounds it: a row passes through
 // some 20 steps, eight of them behind a barrier of its cluster, of which only
-// the load, the first histogram (8 of 47 us per row, about 50 instructions an
-// element) and the list touch every element; registers allow two rows at a
-// time on an SM, so the steps in between leave it half idle (issue slots 46%
-// busy).  One CTA per row that reads its row from L2 again at every pass came
+// the load, the first histogram (about 50 instructions an element) and the list
+// touch every element; registers allow two rows at a time on an SM, 41 us a
+// pair, so the steps in between leave it half idle (issue slots 45% busy).  One CTA per row that reads its row from L2 again at every pass came
 // to the same time with top-k and to 0.5 ms with top-p.
 //
 // Weights are computed in 64 bits (2^y = 2^(j/256) 2^e 2^r with a table of 256
