@@ -193,7 +193,6 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
     const uint32_t q_hi = smem_u32(base), q_lo = q_hi + L::Q, kv0 = q_lo + L::Q;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
-    pdl_trigger();
 
     // ---- which rows: query tiles of all requests in one line, the last first (they see most)
     const int kvh = blockIdx.x % A.n_kv, index = blockIdx.x / A.n_kv, rep = A.n_heads / A.n_kv;
@@ -297,6 +296,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_kv4_prefill(Kv4Args A, int tq,
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
+    // Only now: the GEMMs and GEMVs of this library allocate tensor memory before they wait for the kernel in front of
+    // them, so one that came to lie on this SM first would hold what this CTA still asks for, and wait for it.
+    pdl_trigger();
 
     if (warp < 8) {
         // ================= softmax

@@ -114,3 +114,32 @@ def test_a_model_on_the_paged_cache(ctx):
         tokens = [[int(t)] for t in idx.tolist()]
     assert drawn >= 20 * reqs - 2
     assert host(lens).tolist() == [9 + 19, 4 + 19, 1 + 19] and n_free.item() == pages - 6
+
+
+@pytest.mark.parametrize("hd,rows", [(32, 16), (64, 16), (128, 16), (32, 64), (64, 64)])
+def test_products_right_behind_a_prefill(ctx, hd, rows):
+    """The output projection is launched while the prefill still runs, and both use tensor memory."""
+    import torch
+    rng = np.random.default_rng(hd + rows)
+    heads, n_kv, n, page = 14, 2, 700, 16
+    pages = -(-n // page)
+    cache = torch.zeros(hc.kv4_cache_shape(pages, page, n_kv, hd), dtype=torch.uint8, device="cuda")
+    up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    k, v = (up(rng.standard_normal((n, n_kv, hd)).astype(np.float32)) for _ in range(2))
+    ctx.kv4_append(k, v, torch.arange(n, dtype=torch.int32, device="cuda"), cache)
+    table, lens = torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous(), torch.tensor([n], dtype=torch.int32, device="cuda")
+    row0 = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    cols, kind, out_rows = heads * hd, S.GGML_Q8_0, 896
+    raw = S.gen_weight(kind, out_rows, cols, 7)
+    w = ctx.weight(kind, raw, out_rows, cols)
+    q = up(rng.standard_normal((rows, heads, hd)).astype(np.float32))
+    y, outs = torch.empty(rows, out_rows, device="cuda"), []
+    x = torch.zeros(rows, cols, device="cuda")
+    for _ in range(30):
+        ctx.kv4_attention_prefill(q, cache, table, lens, row0, x.view(rows, heads, hd))
+        (ctx.qgemv if rows <= 16 else ctx.qgemm)(w, x, y)
+        outs.append(y.clone())
+    ctx.check_device_errors()
+    ref = O.qgemv(kind, raw, out_rows, cols, x.cpu().numpy()).reshape(rows, out_rows)
+    for got in outs:
+        assert _rel(got.cpu().numpy(), ref) <= 1e-5
